@@ -25,9 +25,11 @@ LIB = os.path.join(LIBDIR, "libvesper_b200.so")
 SOURCES = ["api.cu", "rope_append.cu", "prefill_f32.cu", "prefill_sm100.cu", "prefill_pair_sm100.cu", "decode_splitkv.cu", "decode_generic.cu", "decode_static.cu",
            "linear_sm100.cu", "block_ops.cu", "decode_exchange.cu", "decode_gqa_mma.cu", "flash_bwd_f32.cu", "attention_f32_sm100.cu",
            "api_hybrid.cu", "sequence_ops.cu", "latent_attention.cu", "latent_prefill_sm100.cu", "latent_decode_mma.cu", "ssd_scan.cu", "ssd_chunk.cu", "ssd_walk_sm100.cu",
-           "sigmoid_attention.cu", "sigmoid_prefill_sm100.cu", "sigmoid_decode_mma.cu", "selective_scan.cu", "moe.cu"]
+           "sigmoid_attention.cu", "sigmoid_prefill_sm100.cu", "sigmoid_decode_mma.cu", "selective_scan.cu", "moe.cu",
+           "api_serving.cu", "qk_norm_rope.cu", "prefill_packed_sm100.cu", "kv4_cache.cu", "decode_kv4.cu"]
 HEADERS = ["common.cuh", "kernels.h", "hybrid.cuh", "f32_tiles.cuh", "cluster_pair.cuh", os.path.join("..", "..", "include", "vesper_b200.h"),
-           os.path.join("..", "..", "include", "vesper_b200_block.h"), os.path.join("..", "..", "include", "vesper_b200_hybrid.h")]
+           os.path.join("..", "..", "include", "vesper_b200_block.h"), os.path.join("..", "..", "include", "vesper_b200_hybrid.h"),
+           "serving.h", "kv4.cuh", os.path.join("..", "..", "include", "vesper_b200_serving.h")]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
