@@ -60,12 +60,16 @@ def quantise(x, exponent=0):
     return torch.where(odd[..., None], torch.full_like(got, math.nan), got).flatten(-2)
 
 
-def attention_bound(o, weighted, size, *, dtype, weights, D):
+def attention_bound(o, weighted, size, *, dtype, weights, D, v):
     """How far a kernel's output may be from 64 bits, element by element: weights rounded to `weights` (each off by half a step, so that the sum moves by at
     most that share of sum p |v|) and the result rounded to `dtype`; and fp32 scores, off by at most D + 8 roundings of 2^-23 of sum |q k| scale (tensor cores
-    truncate), which moves each weight by twice that share."""
+    truncate), which moves each weight by twice that share.
+
+    Weights in fp16 have a smallest step as well, 2^-24: the kernels give the largest weight of the moment 2^7 or more, so that rounding to that step moves a
+    weight of the normalised sum by at most 2^-25 / 2^7 = 2^-32, and the result by 2^-32 of sum |v| over the keys (v, [keys, heads of o, D])."""
     score = (D + 8) * 2.0 ** -23 * size.transpose(0, 1)[..., None] + 2.0 ** -20
-    return unit(dtype) * o.abs() + (unit(weights) + 2 * score) * weighted * (1 + unit(dtype)) + 2.0 ** -30
+    floor = 2.0 ** -32 * v.double().abs().sum(0).repeat_interleave(o.shape[1] // v.shape[1], 0) if weights == torch.float16 else 0
+    return unit(dtype) * o.abs() + (unit(weights) + 2 * score) * weighted * (1 + unit(dtype)) + floor + 2.0 ** -30
 
 
 def lse_bound(lse, size, D):

@@ -164,7 +164,7 @@ def check_packed(q, k, v, o, lse, lens_q, lens_k, scale, causal):
         if nq:
             want, want_lse, weighted, size = R.attention(q[a:a + nq], k[x:x + nk], v[x:x + nk], scale=scale, causal=causal)
             D = q.shape[2]
-            R.check(o[a:a + nq], want, R.attention_bound(want, weighted, size, dtype=q.dtype, weights=q.dtype, D=D), f"o of {nq} on {nk}")
+            R.check(o[a:a + nq], want, R.attention_bound(want, weighted, size, dtype=q.dtype, weights=q.dtype, D=D, v=v[x:x + nk]), f"o of {nq} on {nk}")
             R.check(lse[:, a:a + nq], want_lse, R.lse_bound(want_lse, size, D), f"lse of {nq} on {nk}")
         a += nq
         x += nk
@@ -409,7 +409,7 @@ def check_decode(q, o, lse, k, v, lens, scale, k_new=None, v_new=None, exponents
             kk = torch.cat([kk, R.quantise(k_new[b, :, 0], exponents[0])[None]])
             vv = torch.cat([vv, R.quantise(v_new[b, :, 0], exponents[1])[None]])
         want, want_lse, weighted, size = R.attention(q[b].transpose(0, 1), kk, vv, scale=scale, causal=False)
-        R.check(o[b].transpose(0, 1), want, R.attention_bound(want, weighted, size, dtype=q.dtype, weights=torch.float16, D=D), f"o of sequence {b} with {n} rows")
+        R.check(o[b].transpose(0, 1), want, R.attention_bound(want, weighted, size, dtype=q.dtype, weights=torch.float16, D=D, v=vv), f"o of sequence {b} with {n} rows")
         R.check(lse[b][:, None], want_lse, R.lse_bound(want_lse, size, D), f"lse of sequence {b}")
 
 

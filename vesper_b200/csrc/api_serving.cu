@@ -97,11 +97,23 @@ struct Kv4Plan {
     size_t lens_bytes, total;
 };
 
+// Keys per CTA.  Chosen so that the grid is about `kCtas` per SM for sequences of the longest length.
 Kv4Plan plan_kv4(const vb200_decode_kv4_args* a) {
     Kv4Plan pl{};
     const int most = a->max_len > 0 ? std::min(a->max_len, a->cache.cap) : a->cache.cap;
-    pl.num_splits = 1;
-    pl.chunk = most;
+    int64_t chunk;
+    if (a->num_splits > 0) {
+        chunk = (static_cast<int64_t>(most) + a->num_splits - 1) / a->num_splits;
+    } else {
+        constexpr int kCtas = 3;
+        const int rep = a->Hq / a->Hkv;
+        const int64_t units = static_cast<int64_t>(a->B) * a->Hkv * ((rep + 7) / 8);
+        const int64_t want = std::max<int64_t>(1, kCtas * device_sm_count() / units);
+        chunk = (most + want - 1) / want;
+    }
+    chunk = (chunk + kKv4Tile - 1) / kKv4Tile * kKv4Tile;
+    pl.chunk = static_cast<int>(chunk);
+    pl.num_splits = static_cast<int>((most + chunk - 1) / chunk);
     pl.lens_bytes = up256(sizeof(int) * static_cast<size_t>(a->B));
     pl.total = pl.lens_bytes + up256(sizeof(float) * static_cast<size_t>(a->B) * a->Hq * pl.num_splits * (a->D + 2));
     return pl;

@@ -1,113 +1,433 @@
-// One decode step over a 4-bit key / value cache.
+// One decode step over a 4-bit key / value cache, split over the keys.
 //
 //   s_j = scale q . k_j,  o = sum_j softmax(s)_j v_j,  lse = ln sum_j exp(s_j)     over the rows j < len + appended of the sequence
 // with k_j, v_j as the cache holds them.  A new token is rounded into its row first and attended to as the row says.
+//
+// Grid (split, key head x share of its query heads, sequence); one warp brings tiles of 128 rows by bulk copies into a ring of shared memory (the rows of a
+// head are contiguous: a tile is four copies, codes and scales of keys and of values), four warps take 32 rows of a tile each.  Both products run as warp-level
+// m16n8k16 products, because up to eight query heads share every row:
+//   S [heads, keys] = Q K^T      A = the queries, high halves in rows 0-7 and the rest in rows 8-15, so that a score is as exact as in fp32; B = the keys
+//   O^T [dims, heads] = V^T P^T  A = the values, B = the weights, which stand in the registers of S as this product wants them
+// The order of the summed index is free, so every thread reads its part of a row as it lies: 32 neighbouring elements of a key (one scale), 16 neighbouring
+// elements of four values.  Codes c + 8 become numbers by one and / or and one multiply-add for two of them: the bits 0x6400 | n are the fp16 number 1024 + n,
+// and (1024 + n) s - 1032 s = (n - 8) s is exact in fp16 for every e4m3 scale (s is carried as s / 8, so that 1032 s stays in range).
+//
+// What bounds it: HBM for long caches, 4.25 bits per element, and next to it the instructions that expand them.
 #include "kv4.cuh"
 
 namespace vb200 {
 
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 4;                  // consumers; 32 rows of a tile each
+constexpr int kTile = kKv4Tile;
+constexpr int kThreads = (kWarps + 1) * 32;
+constexpr int kStages = 4;
+constexpr int kMinCtas = 3;
+constexpr int kHeads = 8;                  // query heads of a CTA, at most
 constexpr float kLn2 = 0.6931471805599453f, kLog2e = 1.4426950408889634f;
+constexpr float kRescale = 8.0f;           // weights stay within 2^8 of the running reference,
+constexpr float kLift = 7.0f;              // which weighs 2^7: a weight is then an fp16 number of full precision down to 2^-21 of it, and 2^-32 of it at worst
+static_assert(kTile == kWarps * 32, "32 rows per warp");
 
-// One CTA per (query head, sequence), a warp per row in turn; a lane holds D / 32 elements.
-template <typename T, int D>
-__global__ void __launch_bounds__(kWarps * 32) decode_kv4_kernel(DecodeKv4Params p) {
-    constexpr int kE = D / 32;
-    const int hq = blockIdx.x, b = blockIdx.y, rep = p.Hq / p.Hkv, h = hq / rep;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    __shared__ uint32_t new_codes[2][D / 8];
-    __shared__ uint8_t new_scales[2][D / 32];
-    __shared__ float part[kWarps][D + 2];
+template <int D> struct Layout {
+    static constexpr int kRow = D / 2, kScales = D / 32;                    // bytes of a row
+    static constexpr int kKeyWords = D / 32, kValueWords = D / 64;          // 8-element words of a row that one thread takes
+    static constexpr int kOutTiles = D / 16;
+    static constexpr int kStageBytes = 2 * kTile * (kRow + kScales);
+    static constexpr int kVCodes = kTile * kRow, kKScales = 2 * kTile * kRow, kVScales = kKScales + kTile * kScales;
+    static constexpr int kMerge = kWarps * kHeads * (D + 2) * 4;
+    static constexpr int kRing = kStages * kStageBytes > kMerge ? kStages * kStageBytes : kMerge;
+    static constexpr int kSmem = kRing + 2 * kStages * 8 + 16;
+};
 
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t h2(__half2 x) { return *reinterpret_cast<uint32_t*>(&x); }
+__device__ __forceinline__ __half2 h2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
+__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) { return h2(__hfma2(h2(a), h2(b), h2(c))); }
+
+// the factors of two scales s (one for each half): s / 8, -1032 s / 8, and the same for codes that stand 4 bits higher
+struct Scale2 {
+    uint32_t s, c, s16, c16;
+    __device__ explicit Scale2(uint32_t bytes) {                            // two e4m3 in the low 16 bits
+        const __half2_raw raw = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(bytes), __NV_E4M3);
+        const __half2 t = __half2(raw);
+        s = h2(__hmul2(t, __float2half2_rn(0.125f)));
+        c = h2(__hmul2(t, __float2half2_rn(-129.0f)));
+        s16 = h2(__hmul2(t, __float2half2_rn(0.0078125f)));
+        c16 = h2(__hmul2(t, __float2half2_rn(-9.0f)));
+    }
+};
+// nibbles (j, j + 4) of a word -> x[j] = the numbers (n - 8) s / 8, low and high half
+__device__ __forceinline__ void expand(uint32_t w, const Scale2& f, uint32_t (&x)[4]) {
+    x[0] = hfma2((w & 0x000F000Fu) | 0x64006400u, f.s, f.c);
+    x[1] = hfma2((w & 0x00F000F0u) | 0x64006400u, f.s16, f.c16);
+    const uint32_t u = w >> 8;
+    x[2] = hfma2((u & 0x000F000Fu) | 0x64006400u, f.s, f.c);
+    x[3] = hfma2((u & 0x00F000F0u) | 0x64006400u, f.s16, f.c16);
+}
+
+template <int N> struct Words { uint32_t w[N]; };
+template <int N> __device__ __forceinline__ Words<N> load_words(const unsigned char* p) {
+    Words<N> r;
+    if constexpr (N == 4) { const uint4 v = *reinterpret_cast<const uint4*>(p); r.w[0] = v.x; r.w[1] = v.y; r.w[2] = v.z; r.w[3] = v.w; }
+    else if constexpr (N == 2) { const uint2 v = *reinterpret_cast<const uint2*>(p); r.w[0] = v.x; r.w[1] = v.y; }
+    else r.w[0] = *reinterpret_cast<const uint32_t*>(p);
+    return r;
+}
+
+// Column n of an 8-key tile of S stands for row tile_row(n): with this order the rows that the threads of a warp read at once, keys by columns and values by
+// pairs of columns, lie in different banks (values: two to a bank, instead of four).
+__device__ __forceinline__ int tile_row(int n) { return (n & 4) | ((n & 1) << 1) | (((n >> 1) ^ n) & 1); }
+
+struct Step {
+    int len, total;
+    bool append, overflow;
+};
+__device__ __forceinline__ Step step_of(const DecodeKv4Params& p, int b) {
     const int raw = p.seq_lens ? p.seq_lens[b] : p.uniform_len;
     const long long planned = static_cast<long long>(p.num_splits) * p.chunk;
     const int limit = static_cast<int>(planned < p.cache.cap ? planned : p.cache.cap);
-    const bool overflow = raw < 0 || static_cast<long long>(raw) + p.append > limit;
-    const int len = raw < 0 ? 0 : min(raw, limit);
-    const bool append = p.append && !overflow;
-    if (overflow && hq == 0 && threadIdx.x == 0) atomicCAS(p.status, 0, (2 << 24) | (b & 0xFFFFFF));
-    if (hq == 0 && threadIdx.x == 0) p.lens_used[b] = (len + append) | (append ? 1 << 30 : 0);
-    const long long row0 = b * p.cache.stride_b + h * p.cache.stride_h;
+    Step s;
+    s.overflow = raw < 0 || static_cast<long long>(raw) + p.append > limit;
+    s.len = raw < 0 ? 0 : min(raw, limit);
+    s.append = p.append && !s.overflow;
+    s.total = s.len + s.append;
+    return s;
+}
 
-    if (append && threadIdx.x < 2 * (D / 8)) {
-        const int which = threadIdx.x / (D / 8), w = threadIdx.x % (D / 8);
-        const View4& in = which ? p.v_new : p.k_new;
-        const T* x = static_cast<const T*>(in.ptr) + b * in.sb + h * in.sh + w * 8;
-        float f[8];
-        for (int e = 0; e < 8; ++e) f[e] = Elem<T>::to_f(x[e]);
-        uint8_t s;
-        const uint32_t word = encode8(f, 1.0f / (which ? p.cache.v_unit : p.cache.k_unit), 0xFu << (threadIdx.x & 28), s);
-        new_codes[which][w] = word;
-        if (w % 4 == 0) new_scales[which][w / 4] = s;
-        if (hq % rep == 0) {
-            reinterpret_cast<uint32_t*>(which ? p.cache.v_codes : p.cache.k_codes)[(row0 + len) * (D / 8) + w] = word;
-            if (w % 4 == 0) (which ? p.cache.v_scales : p.cache.k_scales)[(row0 + len) * (D / 32) + w / 4] = s;
-        }
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, kMinCtas) decode_kv4_kernel(DecodeKv4Params p, int head_shares, int direct) {
+    using L = Layout<D>;
+    extern __shared__ __align__(128) unsigned char smem[];
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kRing);
+    uint64_t* empty = full + kStages;
+    int* abort_flag = reinterpret_cast<int*>(empty + kStages);
+
+    const int split = blockIdx.x, h = blockIdx.y / head_shares, share = blockIdx.y % head_shares, b = blockIdx.z;
+    const int rep = p.Hq / p.Hkv, head0 = h * rep + share * kHeads, n_heads = min(kHeads, rep - share * kHeads);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int s = 0; s < kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], kWarps); }
+        *abort_flag = 0;
+        mbar_fence_init();
     }
     __syncthreads();
-
-    float q[kE], acc[kE], m = -INFINITY, l = 0.f;
-    const T* qp = static_cast<const T*>(p.q.ptr) + b * p.q.sb + hq * p.q.sh + lane * kE;
-#pragma unroll
-    for (int e = 0; e < kE; ++e) { q[e] = Elem<T>::to_f(qp[e]); acc[e] = 0.f; }
-    auto value = [&](const uint8_t* codes, const uint8_t* scales, float unit, float (&x)[kE]) {
-        const float s = scale_value(scales[lane * kE / 32]) * unit;
-#pragma unroll
-        for (int e = 0; e < kE; ++e) {
-            const int d = lane * kE + e;
-            x[e] = static_cast<float>(((codes[d / 2] >> (4 * (d & 1))) & 15) - 8) * s;
-        }
-    };
-    for (int j = warp; j < len + append; j += kWarps) {
-        const bool fresh = append && j == len;
-        float k[kE], v[kE];
-        value(fresh ? reinterpret_cast<const uint8_t*>(new_codes[0]) : p.cache.k_codes + (row0 + j) * (D / 2), fresh ? new_scales[0] : p.cache.k_scales + (row0 + j) * (D / 32), p.cache.k_unit, k);
-        value(fresh ? reinterpret_cast<const uint8_t*>(new_codes[1]) : p.cache.v_codes + (row0 + j) * (D / 2), fresh ? new_scales[1] : p.cache.v_scales + (row0 + j) * (D / 32), p.cache.v_unit, v);
-        float s = 0.f;
-#pragma unroll
-        for (int e = 0; e < kE; ++e) s = fmaf(q[e], k[e], s);
-#pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-        s *= p.scale * kLog2e;
-        const float top = fmaxf(m, s), keep = m == -INFINITY ? 0.f : exp2f(m - top), w = exp2f(s - top);
-        l = l * keep + w;
-        m = top;
-#pragma unroll
-        for (int e = 0; e < kE; ++e) acc[e] = fmaf(w, v[e], acc[e] * keep);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const Step st = step_of(p, b);
+    if (split == 0 && blockIdx.y == 0 && tid == 0) {
+        p.lens_used[b] = st.total | (st.append ? 1 << 30 : 0);
+        if (st.overflow) atomicCAS(p.status, 0, (2 << 24) | (b & 0xFFFFFF));
     }
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int begin = split * p.chunk;
+    if (begin >= st.total && !(direct && split == 0)) return;
+    const int end = min(st.total, begin + p.chunk);
+    const int n_tiles = end > begin ? (end - begin + kTile - 1) / kTile : 0;
+    const WaitCtx ctx{abort_flag, p.status};
+    const long long row0 = b * p.cache.stride_b + h * p.cache.stride_h;      // a multiple of 8
+
+    if (warp == kWarps) {
+        // ---- the warp that brings the tiles: up to the last row that the cache held before this step, in whole 16-byte pieces of scales ----
+        if (lane == 0)
+            for (int t = 0; t < n_tiles; ++t) {
+                const int s = t % kStages;
+                if (t >= kStages && !mbar_wait(&empty[s], ((t / kStages) - 1) & 1, ctx, 0x41)) break;
+                const int first = begin + t * kTile;
+                const int rows = min(kTile, (min(end, st.len) - first + 7) & ~7);      // within the capacity: it is a multiple of 8
+                unsigned char* to = smem + s * L::kStageBytes;
+                if (rows <= 0) { mbar_arrive(&full[s]); continue; }                    // the new token alone
+                mbar_arrive_expect_tx(&full[s], 2 * rows * (L::kRow + L::kScales));
+                bulk_load(to, p.cache.k_codes + (row0 + first) * L::kRow, rows * L::kRow, &full[s]);
+                bulk_load(to + L::kKScales, p.cache.k_scales + (row0 + first) * L::kScales, rows * L::kScales, &full[s]);
+                bulk_load(to + L::kVCodes, p.cache.v_codes + (row0 + first) * L::kRow, rows * L::kRow, &full[s]);
+                bulk_load(to + L::kVScales, p.cache.v_scales + (row0 + first) * L::kScales, rows * L::kScales, &full[s]);
+            }
+        return;
+    }
+
+    const int g = lane >> 2, c = lane & 3;
+    // ---- the queries of head g: 32 (or 16) neighbouring elements per thread, brought near one by a power of two, as fp16 and the rest in fp16 ----
+    uint32_t hi[4 * L::kKeyWords], lo[4 * L::kKeyWords];                     // [word][pair j]: elements j and j + 4
+    float q_factor;
+    {
+        float f[8 * L::kKeyWords], top = 0.f;
+        const bool live = g < n_heads;
+        const T* qp = static_cast<const T*>(p.q.ptr) + b * p.q.sb + (head0 + (live ? g : 0)) * p.q.sh + c * (8 * L::kKeyWords);
 #pragma unroll
-    for (int e = 0; e < kE; ++e) part[warp][lane * kE + e] = acc[e];
-    if (lane == 0) { part[warp][D] = m; part[warp][D + 1] = l; }
-    __syncthreads();
-    if (threadIdx.x < D) {
-        float top = -INFINITY, sum = 0.f, o = 0.f;
-        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, part[w][D]);
+        for (int w = 0; w < L::kKeyWords; ++w) {
+            const uint4 v = *reinterpret_cast<const uint4*>(qp + 8 * w);
+            const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 t = Elem<T>::unpack2(u[i]);
+                f[8 * w + 2 * i] = live ? t.x : 0.f;
+                f[8 * w + 2 * i + 1] = live ? t.y : 0.f;
+                top = fmaxf(top, fmaxf(fabsf(f[8 * w + 2 * i]), fabsf(f[8 * w + 2 * i + 1])));
+            }
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+        const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 1), 253);
+        const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23), up = __uint_as_float(static_cast<uint32_t>(e) << 23);
+        q_factor = p.scale * kLog2e * 8.0f * p.cache.k_unit * up;
+#pragma unroll
+        for (int w = 0; w < L::kKeyWords; ++w)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float x = f[8 * w + j] * down, y = f[8 * w + j + 4] * down;
+                const __half2 a = __floats2half2_rn(x, y);
+                const float2 back = __half22float2(a);
+                hi[4 * w + j] = h2(a);
+                lo[4 * w + j] = h2(__floats2half2_rn(x - back.x, y - back.y));
+            }
+    }
+
+    // ---- the new token: rounded by the warp in whose rows it falls; threads [0, D / 8) hold the words of its key, the next D / 8 of its value ----
+    const int new_tile = st.append && st.len >= begin && st.len < end ? (st.len - begin) / kTile : -1;
+    const int new_row = (st.len - begin) % kTile;
+    const bool holds_new = new_tile >= 0 && new_row / 32 == warp;
+    uint32_t new_word = 0;
+    uint8_t new_scale = 0;
+    if (holds_new && lane < 2 * (D / 8)) {
+        const bool value = lane >= D / 8;
+        const int w = lane % (D / 8);
+        const View4& in = value ? p.v_new : p.k_new;
+        const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const T*>(in.ptr) + b * in.sb + h * in.sh + w * 8);
+        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 t = Elem<T>::unpack2(u[i]);
+            x[2 * i] = t.x; x[2 * i + 1] = t.y;
+        }
+        new_word = encode8(x, 1.0f / (value ? p.cache.v_unit : p.cache.k_unit), 0xFu << (lane & 28), new_scale);
+        if (share == 0) {
+            reinterpret_cast<uint32_t*>(value ? p.cache.v_codes : p.cache.k_codes)[(row0 + st.len) * (D / 8) + w] = new_word;
+            if (w % 4 == 0) (value ? p.cache.v_scales : p.cache.k_scales)[(row0 + st.len) * L::kScales + w / 4] = new_scale;
+        }
+    }
+
+    float o[L::kOutTiles][4];                        // [tile][element t or its partner of heads 2c, 2c + 1]
+#pragma unroll
+    for (int i = 0; i < L::kOutTiles; ++i) { o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f; }
+    float m = -INFINITY, l = 0.f;                    // of head g: reference of the weights (log2 units), this thread's share of their sum
+    const int key_row = tile_row(g);
+    for (int t = 0; t < n_tiles; ++t) {
+        const int s = t % kStages;
+        if (!mbar_wait_warp(&full[s], (t / kStages) & 1, ctx, 0x42)) break;
+        unsigned char* tile = smem + s * L::kStageBytes;
+        const int live = end - (begin + t * kTile) - warp * 32;              // rows of this warp's 32 that exist
+        if (live > 0) {
+            if (holds_new && t == new_tile) {
+                if (lane < 2 * (D / 8)) {
+                    const bool value = lane >= D / 8;
+                    const int w = lane % (D / 8);
+                    *reinterpret_cast<uint32_t*>(tile + (value ? L::kVCodes : 0) + new_row * L::kRow + w * 4) = new_word;
+                    if (w % 4 == 0) tile[(value ? L::kVScales : L::kKScales) + new_row * L::kScales + w / 4] = new_scale;
+                }
+                __syncwarp();
+            }
+            const unsigned char* k_codes = tile + warp * 32 * L::kRow + c * (4 * L::kKeyWords);
+            const unsigned char* k_scales = tile + L::kKScales + warp * 32 * L::kScales + (D == 128 ? c : c >> 1);
+            float sc[4][4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+                const int row = n * 8 + key_row;
+                const Words<L::kKeyWords> k = load_words<L::kKeyWords>(k_codes + row * L::kRow);
+                const Scale2 f(static_cast<uint32_t>(k_scales[row * L::kScales]) * 0x0101u);
+#pragma unroll
+                for (int w = 0; w < L::kKeyWords; ++w) {
+                    uint32_t x[4];
+                    expand(k.w[w], f, x);
+                    mma(sc[n], hi[4 * w], lo[4 * w], hi[4 * w + 1], lo[4 * w + 1], x[0], x[1]);
+                    mma(sc[n], hi[4 * w + 2], lo[4 * w + 2], hi[4 * w + 3], lo[4 * w + 3], x[2], x[3]);
+                }
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    float x = (sc[n][j] + sc[n][j + 2]) * q_factor;
+                    if (live < 32 && n * 8 + tile_row(2 * c + j) >= live) x = -INFINITY;
+                    sc[n][j] = x;
+                    top = fmaxf(top, x);
+                }
+            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+            const bool grow = top > m + kRescale;
+            if (__any_sync(0xFFFFFFFFu, grow)) {
+                const float next = grow ? top : m;
+                const float keep = m == -INFINITY ? 0.f : fast_exp2(m - next);
+                l *= keep;
+                m = next;
+                const float k0 = __shfl_sync(0xFFFFFFFFu, keep, 8 * c), k1 = __shfl_sync(0xFFFFFFFFu, keep, 8 * c + 4);
+#pragma unroll
+                for (int i = 0; i < L::kOutTiles; ++i) { o[i][0] *= k0; o[i][1] *= k1; o[i][2] *= k0; o[i][3] *= k1; }
+            }
+            const float zero = m == -INFINITY ? 0.f : m - kLift;              // every score so far -infinity: weights of zero
+            uint32_t weight[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const float x = fast_exp2(sc[n][0] - zero), y = fast_exp2(sc[n][1] - zero);
+                l += x + y;
+                weight[n] = h2(__floats2half2_rn(x, y));
+            }
+            const unsigned char* v_codes = tile + L::kVCodes + warp * 32 * L::kRow + g * (4 * L::kValueWords);
+            const unsigned char* v_scales = tile + L::kVScales + warp * 32 * L::kScales + (D == 128 ? g >> 1 : g >> 2);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                if (u * 16 >= live) break;
+                // rows of columns 2c, 2c + 1 of both 8-key tiles: [0][.] of the first, [1][.] of the second
+                uint32_t x[2][2 * L::kValueWords][4];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int ra = u * 16 + half * 8 + tile_row(2 * c), rb = u * 16 + half * 8 + tile_row(2 * c + 1);
+                    const Words<L::kValueWords> a = load_words<L::kValueWords>(v_codes + ra * L::kRow), bw = load_words<L::kValueWords>(v_codes + rb * L::kRow);
+                    uint32_t sa = v_scales[ra * L::kScales], sb = v_scales[rb * L::kScales];
+                    if (live < 32) {                                          // rows behind the last one: anything may stand there, NaN scales too
+                        if (ra >= live) sa = 0;
+                        if (rb >= live) sb = 0;
+                    }
+                    const Scale2 f(sa | (sb << 8));
+#pragma unroll
+                    for (int w = 0; w < L::kValueWords; ++w) {
+                        expand(__byte_perm(a.w[w], bw.w[w], 0x5410), f, x[half][2 * w]);
+                        expand(__byte_perm(a.w[w], bw.w[w], 0x7632), f, x[half][2 * w + 1]);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < L::kOutTiles; ++i) {
+                    // D = 128: rows of the tile are elements i and 8 + i of this thread's 16; D = 64: i and 4 + i of its 8
+                    const int w0 = D == 128 ? i / 4 : 0, w1 = D == 128 ? 2 + i / 4 : 1, j = i % 4;
+                    mma(o[i], x[0][w0][j], x[0][w1][j], x[1][w0][j], x[1][w1][j], weight[2 * u], weight[2 * u + 1]);
+                }
+            }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[s]);
+    }
+
+    if (*ctx.abort_flag) {                           // copies of an abandoned tile may still be landing: far longer than one takes
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000LL) {}
+    }
+
+    // ---- merge the warps through shared memory (the ring is free once all of them are here) ----
+    l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
+    l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
+    asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
+    float* part = reinterpret_cast<float*>(smem);                            // [warp][head][D + 2]
+#pragma unroll
+    for (int i = 0; i < L::kOutTiles; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int d = D == 128 ? 16 * g + i + 8 * (e >> 1) : 8 * g + i + 4 * (e >> 1);
+            part[(warp * kHeads + 2 * c + (e & 1)) * (D + 2) + d] = o[i][e];
+        }
+    if (c == 0) { part[(warp * kHeads + g) * (D + 2) + D] = m - kLift; part[(warp * kHeads + g) * (D + 2) + D + 1] = l; }
+    asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
+    for (int i = tid; i < n_heads * D; i += kWarps * 32) {
+        const int r = i / D, d = i % D;
+        float top = -INFINITY, sum = 0.f, acc = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, part[(w * kHeads + r) * (D + 2) + D]);
+#pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-            const float f = part[w][D] == -INFINITY ? 0.f : exp2f(part[w][D] - top);
-            sum += part[w][D + 1] * f;
-            o += part[w][threadIdx.x] * f;
+            const float* rec = part + (w * kHeads + r) * (D + 2);
+            const float f = rec[D] == -INFINITY ? (rec[D + 1] == 0.f ? 0.f : rec[D + 1]) : fast_exp2(rec[D] - top);      // (no reference, a sum that is NaN: NaN)
+            sum += rec[D + 1] * f;
+            acc += rec[d] * f;
         }
-        static_cast<T*>(p.o.ptr)[b * p.o.sb + hq * p.o.sh + threadIdx.x] = Elem<T>::from_f(sum == 0.f ? 0.f : o / sum);
-        if (p.lse && threadIdx.x == 0) p.lse[b * p.Hq + hq] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+        const float value = sum == 0.f ? 0.f : acc / sum * (8.0f * p.cache.v_unit);
+        const int hq = head0 + r;
+        if (direct) {
+            static_cast<T*>(p.o.ptr)[b * p.o.sb + hq * p.o.sh + d] = Elem<T>::from_f(value);
+            if (p.lse && d == 0) p.lse[b * p.Hq + hq] = sum == 0.f ? -INFINITY : (top + fast_log2(sum)) * kLn2;
+        } else {
+            float* rec = p.partials + ((static_cast<long long>(b) * p.Hq + hq) * p.num_splits + split) * (D + 2);
+            rec[d] = value;
+            if (d == 0) { rec[D] = top; rec[D + 1] = sum; }
+        }
     }
 }
 
-__global__ void advance_kernel(DecodeKv4Params p) {
-    const int b = blockIdx.x * blockDim.x + threadIdx.x;
-    if (b < p.B && StepLen::header_appended(p.lens_used[b])) p.seq_lens[b] = StepLen::header_total(p.lens_used[b]);
+// Merges the splits of a query head: o = sum_i o_i l_i 2^(m_i - m) / sum_i l_i 2^(m_i - m); stores the advanced length.  512 threads: 512 / D groups of splits.
+constexpr int kCombineThreads = 512;
+template <typename T, int D>
+__global__ void __launch_bounds__(kCombineThreads) decode_kv4_combine_kernel(DecodeKv4Params p) {
+    constexpr int kGroups = kCombineThreads / D;
+    __shared__ float sum_of[kGroups][D], l_of[kGroups];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int hq = blockIdx.x, b = blockIdx.y, d = threadIdx.x % D, group = threadIdx.x / D;
+    const int used = p.lens_used[b], total = StepLen::header_total(used);
+    if (p.advance_lens && hq == 0 && threadIdx.x == 0 && StepLen::header_appended(used)) p.seq_lens[b] = total;
+    const int n = (total + p.chunk - 1) / p.chunk;
+    const float* rec = p.partials + (static_cast<long long>(b) * p.Hq + hq) * p.num_splits * (D + 2);
+    float top = -INFINITY;
+    for (int i = threadIdx.x & 31; i < n; i += 32) top = fmaxf(top, rec[i * (D + 2) + D]);
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    float acc = 0.f, sum = 0.f;
+    for (int i = group; i < n; i += kGroups) {
+        const float m = rec[i * (D + 2) + D], l = rec[i * (D + 2) + D + 1];
+        const float f = (m == -INFINITY && l == 0.f) ? 0.f : l * fast_exp2(m == -INFINITY ? 0.f : m - top);
+        acc = fmaf(f, rec[i * (D + 2) + d], acc);
+        sum += f;
+    }
+    sum_of[group][d] = acc;
+    if (d == 0) l_of[group] = sum;
+    __syncthreads();
+    if (group == 0) {
+        acc = 0.f; sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i) { acc += sum_of[i][d]; sum += l_of[i]; }
+        static_cast<T*>(p.o.ptr)[b * p.o.sb + hq * p.o.sh + d] = Elem<T>::from_f(sum == 0.f ? 0.f : acc / sum);
+        if (p.lse && d == 0) p.lse[b * p.Hq + hq] = sum == 0.f ? -INFINITY : (top + fast_log2(sum)) * kLn2;
+    }
+}
+
+template <typename F, typename... Args>
+cudaError_t launch_dependent(F kernel, dim3 grid, int threads, size_t smem, cudaStream_t s, Args... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 template <typename T, int D>
 int launch_t(cudaStream_t s, const DecodeKv4Params& p) {
-    decode_kv4_kernel<T, D><<<dim3(p.Hq, p.B), kWarps * 32, 0, s>>>(p);
+    static thread_local bool configured[64] = {};      // per device ordinal: the attribute belongs to the device's context
+    int dev = 0;
+    VB200_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64) return set_detail(VB200_ERR_NO_DEVICE, "device ordinal out of range");
+    if (!configured[dev]) {
+        VB200_CUDA_TRY(cudaFuncSetAttribute(decode_kv4_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::kSmem));
+        configured[dev] = true;
+    }
+    const int rep = p.Hq / p.Hkv, shares = (rep + kHeads - 1) / kHeads;
+    const int advance = p.advance_lens && p.append, direct = p.num_splits == 1 && !advance;
+    profile_mark_begin(s);
+    VB200_CUDA_TRY(launch_dependent(decode_kv4_kernel<T, D>, dim3(p.num_splits, p.Hkv * shares, p.B), kThreads, Layout<D>::kSmem, s, p, shares, direct));
+    profile_mark_end(s);
     note_launch();
-    if (p.advance_lens && p.seq_lens && p.append) {
-        advance_kernel<<<(p.B + 127) / 128, 128, 0, s>>>(p);
+    if (!direct) {
+        VB200_CUDA_TRY(launch_dependent(decode_kv4_combine_kernel<T, D>, dim3(p.Hq, p.B), kCombineThreads, 0, s, p));
         note_launch();
     }
-    VB200_CUDA_TRY(cudaPeekAtLastError());
     return VB200_OK;
 }
 

@@ -66,6 +66,7 @@ int launch_kv4_append(cudaStream_t s, const Kv4RowsParams& p);
 int launch_kv4_read(cudaStream_t s, const Kv4RowsParams& p);
 
 // ---- decode_kv4.cu ----
+constexpr int kKv4Tile = 128;              // rows that a CTA takes at a time: chunks are multiples of it
 struct DecodeKv4Params {
     int dtype, B, Hq, Hkv, D;
     float scale;
