@@ -455,6 +455,18 @@ def test_decode_kv4_long(S, lens):
     run_decode(S, rng(1), len(lens), 16, 2, 128, torch.bfloat16, lens, append=True, max_len=max(lens) + 1)
 
 
+@pytest.mark.parametrize("B, Hkv, most", [(1, 8, 9000), (37, 4, 1500), (1300, 1, 700), (3, 2, 40000)])
+def test_decode_kv4_ragged(S, B, Hkv, most):
+    """Lengths of every size in one batch, empty sequences among them, the work shared out over the device."""
+    r = np.random.RandomState(B)
+    lens = [int(x) for x in np.exp(r.uniform(0, math.log(most), B))]
+    for i in range(0, B, 7):
+        lens[i] = 0 if B > 1 else most
+    lens[-1] = most
+    run_decode(S, rng(B), B, 4 * Hkv, Hkv, 64, torch.bfloat16, lens, append=True, advance=True)
+    run_decode(S, rng(B), B, 4 * Hkv, Hkv, 128, torch.bfloat16, lens)
+
+
 def test_decode_kv4_exponents_and_large_queries(S):
     run_decode(S, rng(2), 2, 8, 2, 128, torch.bfloat16, [150, 31], append=True, exponents=(5, -7))
     run_decode(S, rng(3), 2, 8, 2, 128, torch.bfloat16, [150, 31], q_scale=30.0)

@@ -93,29 +93,31 @@ int kv4_rows(const vb200_kv4_rows_args* a, bool writing) {
 }
 
 struct Kv4Plan {
-    int num_splits, chunk;
+    int limit, per_unit, ctas, share;
+    int64_t units, tiles;                  // of the batch, and of its longest sequence
     size_t lens_bytes, total;
 };
 
-// Keys per CTA.  Chosen so that the grid is about `kCtas` per SM for sequences of the longest length.
+// A CTA per unit (a key head of a sequence with up to eight query heads) while no sequence has more than two tiles: nothing is left to merge.  Else two CTAs
+// per SM share the row of all tiles.  num_splits: pieces of that part of the longest sequence, and as many CTAs as these may need.
 Kv4Plan plan_kv4(const vb200_decode_kv4_args* a) {
     Kv4Plan pl{};
-    const int most = a->max_len > 0 ? std::min(a->max_len, a->cache.cap) : a->cache.cap;
-    int64_t chunk;
+    pl.limit = a->max_len > 0 ? std::min(a->max_len, a->cache.cap) : a->cache.cap;
+    pl.units = static_cast<int64_t>(a->B) * a->Hkv * ((a->Hq / a->Hkv + 7) / 8);
+    pl.tiles = (static_cast<int64_t>(pl.limit) + kKv4Tile - 1) / kKv4Tile;
+    int64_t ctas;
     if (a->num_splits > 0) {
-        chunk = (static_cast<int64_t>(most) + a->num_splits - 1) / a->num_splits;
+        pl.per_unit = a->num_splits == 1;
+        const int64_t share = (pl.tiles + a->num_splits - 1) / a->num_splits;
+        ctas = pl.per_unit ? pl.units : pl.units * ((pl.tiles + share - 1) / share);
+        pl.share = static_cast<int>(share);
     } else {
-        constexpr int kCtas = 3;
-        const int rep = a->Hq / a->Hkv;
-        const int64_t units = static_cast<int64_t>(a->B) * a->Hkv * ((rep + 7) / 8);
-        const int64_t want = std::max<int64_t>(1, kCtas * device_sm_count() / units);
-        chunk = (most + want - 1) / want;
+        pl.per_unit = pl.tiles <= 2;
+        ctas = pl.per_unit ? pl.units : std::min<int64_t>(2 * device_sm_count(), pl.units * pl.tiles);
     }
-    chunk = (chunk + kKv4Tile - 1) / kKv4Tile * kKv4Tile;
-    pl.chunk = static_cast<int>(chunk);
-    pl.num_splits = static_cast<int>((most + chunk - 1) / chunk);
-    pl.lens_bytes = up256(sizeof(int) * static_cast<size_t>(a->B));
-    pl.total = pl.lens_bytes + up256(sizeof(float) * static_cast<size_t>(a->B) * a->Hq * pl.num_splits * (a->D + 2));
+    pl.ctas = static_cast<int>(std::min<int64_t>(ctas, INT32_MAX));
+    pl.lens_bytes = up256(sizeof(int) * (2 * static_cast<size_t>(a->B) + 1));
+    pl.total = pl.lens_bytes + (pl.per_unit ? 0 : up256(sizeof(float) * (pl.units + ctas) * 8 * (a->D + 2)));
     return pl;
 }
 
@@ -225,8 +227,8 @@ size_t vb200_decode_kv4_workspace_bytes_max(const vb200_decode_kv4_args* a) {
     if (!plannable(a)) return 0;
     vb200_decode_kv4_args t = *a;
     size_t most = 0;
-    for (int n = 1; n <= a->cache.cap; ++n) {
-        t.max_len = n;
+    for (int64_t n = 1; n < a->cache.cap + kKv4Tile; n += kKv4Tile) {        // the plan goes by whole tiles
+        t.max_len = static_cast<int>(std::min<int64_t>(n, a->cache.cap));
         most = std::max(most, plan_kv4(&t).total);
     }
     return most;
@@ -251,6 +253,7 @@ int vb200_decode_kv4_fwd(const vb200_decode_kv4_args* a) {
         (append && (!view_aligned(used(a->k_new, a->B, a->Hkv, 1), 2) || !view_aligned(used(a->v_new, a->B, a->Hkv, 1), 2))))
         return set_detail(VB200_ERR_ALIGNMENT, "q / k_new / v_new / o base and strides must be 16-byte aligned");
     const Kv4Plan pl = plan_kv4(a);
+    if (pl.units * pl.tiles > INT32_MAX || a->cache.cap >= 1 << 30) return set_detail(VB200_ERR_INVALID_ARG, "4-bit decode: too many rows in one call");
     if (!a->workspace || a->workspace_bytes < pl.total) return set_detail(VB200_ERR_WORKSPACE, "decode workspace too small (see vb200_decode_kv4_workspace_bytes)");
     if (reinterpret_cast<uintptr_t>(a->workspace) % 256 != 0) return set_detail(VB200_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
     DeviceGuard g;
@@ -263,10 +266,11 @@ int vb200_decode_kv4_fwd(const vb200_decode_kv4_args* a) {
     p.v_new = used_view(a->v_new, a->B, a->Hkv, 1);
     p.lse = a->lse;
     p.cache = cache_view(a->cache, a->Hkv);
-    p.seq_lens = a->seq_lens; p.uniform_len = a->uniform_len; p.advance_lens = a->advance_lens; p.append = append;
-    p.num_splits = pl.num_splits; p.chunk = pl.chunk;
+    p.seq_lens = a->seq_lens; p.uniform_len = a->uniform_len; p.advance_lens = a->advance_lens && append; p.append = append;
+    p.limit = pl.limit; p.per_unit = pl.per_unit; p.ctas = pl.ctas; p.share = pl.share;
     p.lens_used = static_cast<int*>(a->workspace);
-    p.partials = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + pl.lens_bytes);
+    p.tiles_before = p.lens_used + a->B;
+    p.records = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + pl.lens_bytes);
     if (int rc = status_or_fail(p.status)) return rc;
     return launch_decode_kv4(static_cast<cudaStream_t>(a->stream), p);
 }

@@ -66,7 +66,7 @@ int launch_kv4_append(cudaStream_t s, const Kv4RowsParams& p);
 int launch_kv4_read(cudaStream_t s, const Kv4RowsParams& p);
 
 // ---- decode_kv4.cu ----
-constexpr int kKv4Tile = 128;              // rows that a CTA takes at a time: chunks are multiples of it
+constexpr int kKv4Tile = 256;              // rows that a CTA takes at a time: chunks are multiples of it
 struct DecodeKv4Params {
     int dtype, B, Hq, Hkv, D;
     float scale;
@@ -75,9 +75,11 @@ struct DecodeKv4Params {
     Kv4View cache;
     int* seq_lens;
     int uniform_len, advance_lens, append;
-    int num_splits, chunk;
-    float* partials;                       // [B, Hq, num_splits, D + 2]: O / l, m, l
-    int* lens_used;                        // [B]: StepLen::header of each sequence
+    int limit;                             // rows that a sequence may have after the step
+    int per_unit, ctas, share;             // a CTA per unit, or the row of tiles in pieces of `share` (0: an equal part for each CTA)
+    int* lens_used;                        // [B]: total rows | appended << 30
+    int* tiles_before;                     // [B + 1]: tiles of the sequences before this one; last: the share
+    float* records;                        // [ctas + units, 8, D + 2]: O / l, m, l of a CTA's part of a unit
     int* status;
 };
 int launch_decode_kv4(cudaStream_t s, const DecodeKv4Params& p);
