@@ -134,6 +134,9 @@ int check_packed(const vb200_prefill_packed_args* a) {
     if (!a->q.ptr || !a->o.ptr || (a->total_k > 0 && (!a->k.ptr || !a->v.ptr))) return set_detail(VB200_ERR_INVALID_ARG, "q, k, v, o must be non-null");
     if (!a->cu_seqlens_q) return set_detail(VB200_ERR_INVALID_ARG, "cu_seqlens_q must be non-null");
     if (!countable(1, a->total_q, a->Hq) || a->batch > 65536) return set_detail(VB200_ERR_INVALID_ARG, "packed attention: at most 2^31 - 1 (token, head) pairs and 65536 sequences");
+    auto dense = [](const vb200_tensor4& t, int H, int tokens) { return (H == 1 || t.stride_h > 0) && (tokens <= 1 || t.stride_s > 0); };
+    if (!dense(a->q, a->Hq, a->total_q) || !dense(a->o, a->Hq, a->total_q) || !dense(a->k, a->Hkv, a->total_k) || !dense(a->v, a->Hkv, a->total_k))
+        return set_detail(VB200_ERR_UNSUPPORTED, "packed attention: strides must be positive (no broadcast heads or tokens)");
     const bool k_ok = a->total_k == 0 || (view_aligned(used(a->k, 1, a->Hkv, a->total_k), 2) && view_aligned(used(a->v, 1, a->Hkv, a->total_k), 2));
     if (!view_aligned(used(a->q, 1, a->Hq, a->total_q), 2) || !view_aligned(used(a->o, 1, a->Hq, a->total_q), 2) || !k_ok)
         return set_detail(VB200_ERR_ALIGNMENT, "q / k / v / o base and strides must be 16-byte aligned");

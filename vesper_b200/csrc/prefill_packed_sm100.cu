@@ -1,75 +1,645 @@
-// Attention over packed prompts.
+// Attention over packed prompts on the tensor cores.
 //
 //   s_ij = scale q_i . k_j,  key j of n_k visible to query i of n_q iff j <= n_k - n_q + i (causal) or always
 //   O_i = sum_j softmax_j(s_ij) v_j,  LSE_i = ln sum_j exp(s_ij);  zeros and -infinity where no key is visible
+//
+// A tile is 128 rows: 128 / F tokens of one sequence by F heads of one key head's group (F: the power of two of the group, at most 16), row = token * F +
+// head, as one TMA box of q brings them.  Short sequences fill a tile with heads instead of padding, and the rows of a tile see nearly the same keys.  A work
+// item is two tiles of neighbouring tokens that read the same blocks of 128 keys.  The lengths are on the device: a first kernel lists the items with the
+// longest first, then persistent CTAs, one per SM, take them in snake order.
+//   warps 0-3    softmax and epilogue of tile 0, a row per thread (TMEM lane)
+//   warps 4-7    the same for tile 1
+//   warp  8      TMA: q tiles (3 buffers, so that the next item's come while this one computes) and the ring of key and value blocks
+//   warp  9      tcgen05.mma issuer, TMEM owner
+// TMEM (512 columns): S0 [0,128) S1 [128,256) O0 [256,256+D) O1 [384,384+D); the weights (16 bits, two to a column) overwrite the first 64 columns of their S.
+// The last block of a tile takes only the columns (by 32) and the rows of V (by 16) that a row of it can see.  The rows of V behind the sequence in its last
+// 16 are another sequence's, or nobody's: they are cleared in shared memory, since a weight of zero does not silence a NaN.
+// Every wait is bounded (mbar_wait); on expiry the CTA drains and returns with the status word set.
+#include "hybrid.cuh"
 #include "serving.h"
+
+#include <algorithm>
+#include <cstdio>
 
 namespace vb200 {
 
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kBlockM = 128, kBlockN = 128;
+constexpr int kStages = 4;                 // key / value slots
+constexpr int kQBufs = 3;
+constexpr int kProducerWarp = 8, kMmaWarp = 9;
+constexpr int kThreads = 384;              // three warpgroups: registers are moved by warpgroups
 constexpr float kLn2 = 0.6931471805599453f, kLog2e = 1.4426950408889634f;
+constexpr float kRescale = 8.0f;           // weights stay within 2^8 of the running reference
+constexpr float kLift = 7.0f;              // which weighs 2^7, so that fp16 weights keep their precision down to 2^-21 of it
+constexpr int kRegSoftmax = 216, kRegOther = 72;
+static_assert(kRegSoftmax * 256 + kRegOther * 128 <= 168 * 384, "register budget");
+
+// Two tiles of neighbouring tokens of a sequence, without the head block: tokens [q0, q0 + tokens), keys [k0, k0 + keys), of which the last that token i
+// sees is `last` + i (causal).
+struct alignas(16) Item {
+    int q0, tokens, k0, keys;
+    int last, blocks[2], pad;              // key blocks of each tile
+};
+
+struct Plan {                              // workspace: the header, the items, the first item of each sequence
+    int items;
+};
+
+struct Shape {
+    int fold, tokens;                      // heads and tokens of a tile
+    int head_blocks;                       // of the model
+    int max_items;                         // without head blocks
+};
+Shape shape_of(int batch, int Hq, int Hkv, int total_q) {
+    Shape s;
+    const int rep = Hq / Hkv;
+    s.fold = 1;
+    while (s.fold < 16 && rep % (2 * s.fold) == 0) s.fold *= 2;
+    s.tokens = kBlockM / s.fold;
+    s.head_blocks = Hq / s.fold;
+    s.max_items = total_q / (2 * s.tokens) + batch;
+    return s;
+}
+
+// ---- the list of items, by descending number of key blocks ----
+constexpr int kPlanThreads = 1024, kBins = 1024;
+
+__device__ __forceinline__ int bin_of(int blocks) {      // longest first
+    return kBins - 1 - (blocks < 512 ? blocks : 512 + min(511, (blocks - 512) >> 4));
+}
 
 struct Sequence {
     int q0, nq, k0, nk;
 };
+// a sequence whose offsets are not in order or not within the tokens is left out
 __device__ __forceinline__ Sequence sequence_of(const PackedParams& p, int i) {
     const int a = p.cu_q[i], b = p.cu_q[i + 1], x = p.cu_k[i], y = p.cu_k[i + 1];
     const bool ok = a >= 0 && a <= b && b <= p.total_q && x >= 0 && x <= y && y <= p.total_k;
     return ok ? Sequence{a, b - a, x, y - x} : Sequence{0, 0, 0, 0};
 }
 
-// a warp per (token, query head): the keys one after the other, D / 32 elements per lane
+__global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedParams p, int tile_tokens, int max_items, Plan* plan, Item* items, int* first_item) {
+    __shared__ int hist[kBins];
+    __shared__ int warp_sum[32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, pair = 2 * tile_tokens;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the attention kernel sets itself up meanwhile, and waits for this one
+    hist[tid] = 0;
+    // first item of each sequence: every thread a piece of the sequences, then a sum over the threads before it
+    const int per = (p.batch + kPlanThreads - 1) / kPlanThreads, i0 = min(tid * per, p.batch), i1 = min(i0 + per, p.batch);
+    int mine = 0;
+    for (int i = i0; i < i1; ++i) mine += (sequence_of(p, i).nq + pair - 1) / pair;
+    auto scan = [&](int x) {                             // inclusive, over the block
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) warp_sum[warp] = x;
+        __syncthreads();
+        if (warp == 0) {
+            int y = warp_sum[lane];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int z = __shfl_up_sync(0xFFFFFFFFu, y, o);
+                if (lane >= o) y += z;
+            }
+            warp_sum[lane] = y;
+        }
+        __syncthreads();
+        const int before = warp > 0 ? warp_sum[warp - 1] : 0;
+        __syncthreads();
+        return x + before;
+    };
+    int next = scan(mine) - mine;
+    for (int i = i0; i < i1; ++i) {
+        first_item[i] = next;
+        next += (sequence_of(p, i).nq + pair - 1) / pair;
+    }
+    if (i1 == p.batch && i0 < i1) {
+        first_item[p.batch] = next;
+        plan->items = min(next, max_items);              // (offsets in order leave no more than max_items)
+    }
+    __syncthreads();
+    const int n = min(first_item[p.batch], max_items);
+    auto item_at = [&](int idx) {
+        int lo = 0, hi = p.batch;                        // the last sequence whose first item is at or before idx
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (first_item[mid] <= idx) lo = mid; else hi = mid;
+        }
+        const Sequence s = sequence_of(p, lo);
+        const int r0 = (idx - first_item[lo]) * pair;
+        Item w;
+        w.q0 = s.q0 + r0;
+        w.tokens = min(pair, s.nq - r0);
+        w.k0 = s.k0;
+        w.keys = s.nk;
+        w.last = p.causal ? s.nk - s.nq + r0 : s.nk - 1;
+        w.pad = 0;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int end = p.causal ? min(s.nk, w.last + min(w.tokens, (t + 1) * tile_tokens)) : s.nk;
+            w.blocks[t] = w.tokens > t * tile_tokens && end > 0 ? (end + kBlockN - 1) / kBlockN : 0;
+        }
+        return w;
+    };
+    for (int idx = tid; idx < n; idx += kPlanThreads) {
+        const Item w = item_at(idx);
+        atomicAdd(&hist[bin_of(max(w.blocks[0], w.blocks[1]))], 1);
+    }
+    __syncthreads();
+    const int count = hist[tid];
+    const int at = scan(count) - count;
+    hist[tid] = at;
+    __syncthreads();
+    for (int idx = tid; idx < n; idx += kPlanThreads) {  // (the order within a bin is free: results do not depend on it)
+        const Item w = item_at(idx);
+        items[atomicAdd(&hist[bin_of(max(w.blocks[0], w.blocks[1]))], 1)] = w;
+    }
+}
+
+// ---- the attention kernel ----
+struct __align__(8) Barriers {
+    uint64_t q_full[kQBufs], q_free[kQBufs];
+    uint64_t kv_full[kStages], kv_empty[kStages];
+    uint64_t s_full[2], p_ready[2], o_done[2];
+    uint64_t mma_done;
+    uint32_t tmem_base;
+    int abort_flag;
+};
+
+struct TmaMaps {
+    CUtensorMap q, k, v;
+};
+
+template <int D>
+struct Cfg {
+    static constexpr int kHalves = D / 64;                       // 64-column (128-byte) boxes per row
+    static constexpr int kHalfBytes = 128 * 128;                 // one [128 rows][64 cols] 16-bit box
+    static constexpr int kTileBytes = kHalves * kHalfBytes;
+    static constexpr int kSmemBytes = (kQBufs + kStages) * kTileBytes + 1024 /*alignment slack*/ + 256 /*Barriers*/;
+};
+static_assert(sizeof(Barriers) <= 256, "room for the barriers");
+
+// Round r gives CTA c item r * G + c (even r) or r * G + G - 1 - c (odd r), which evens out the sums.  -1: none.
+__device__ __forceinline__ int item_of_round(int round, int n_items) {
+    const int G = gridDim.x, c = blockIdx.x;
+    const int idx = round * G + ((round & 1) ? (G - 1 - c) : c);
+    return idx < n_items ? idx : -1;
+}
+
+template <int N> __device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
 template <typename T, int D>
-__global__ void __launch_bounds__(kWarps * 32) prefill_packed_kernel(PackedParams p) {
-    constexpr int kE = D / 32;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int token = blockIdx.x * kWarps + warp, hq = blockIdx.y, h = hq / (p.Hq / p.Hkv);
-    if (token >= p.total_q) return;
-    Sequence s{0, 0, 0, 0};
-    for (int i = 0; i < p.batch; ++i) {
-        const Sequence c = sequence_of(p, i);
-        if (token >= c.q0 && token < c.q0 + c.nq) { s = c; break; }
+__global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __grid_constant__ TmaMaps maps, PackedParams p, Shape shape, const Plan* plan, const Item* items) {
+    using C = Cfg<D>;
+    extern __shared__ unsigned char smem_dyn[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));      // 128B-swizzled tiles
+    unsigned char* q_smem = smem;                                   // kQBufs tiles
+    unsigned char* kv_smem = smem + kQBufs * C::kTileBytes;         // kStages tiles
+    Barriers* bar = reinterpret_cast<Barriers*>(smem + (kQBufs + kStages) * C::kTileBytes);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    // ---- setup ----
+    if (warp == kMmaWarp) {
+        if (lane == 0) {
+            for (int b = 0; b < kQBufs; ++b) { mbar_init(&bar->q_full[b], 1); mbar_init(&bar->q_free[b], 1); }
+            for (int t = 0; t < 2; ++t) { mbar_init(&bar->s_full[t], 1); mbar_init(&bar->p_ready[t], kBlockM); mbar_init(&bar->o_done[t], 1); }
+            for (int s = 0; s < kStages; ++s) { mbar_init(&bar->kv_full[s], 1); mbar_init(&bar->kv_empty[s], 1); }
+            mbar_init(&bar->mma_done, 1);
+            bar->abort_flag = 0;
+            mbar_fence_init();
+        }
+        __syncwarp();
+        tmem_alloc(&bar->tmem_base, 512);
+        tmem_relinquish();
+        tc_fence_before();
+    } else if (warp == kProducerWarp && lane == 0) {
+        tma_prefetch_desc(&maps.q); tma_prefetch_desc(&maps.k); tma_prefetch_desc(&maps.v);
     }
-    if (s.nq == 0) return;
-    const int n = p.causal ? min(s.nk, s.nk - s.nq + (token - s.q0) + 1) : s.nk;
-    float q[kE], acc[kE], m = -INFINITY, l = 0.f;
-    const T* qp = static_cast<const T*>(p.q.ptr) + hq * p.q.sh + token * p.q.ss + lane * kE;
+    __syncthreads();
+    tc_fence_after();
+    asm volatile("griddepcontrol.wait;" ::: "memory");              // the list of items
+    const uint32_t tmem_base = bar->tmem_base;
+    const WaitCtx abort_flag{&bar->abort_flag, p.status};
+    const int n_items = plan->items * shape.head_blocks;
+    const int n_rounds = (n_items + gridDim.x - 1) / gridDim.x;
+    const int rep = p.Hq / p.Hkv;
+    auto item_of = [&](int idx) {
+        Item w;
+        const int4* src = reinterpret_cast<const int4*>(items + idx / shape.head_blocks);
+        int4* dst = reinterpret_cast<int4*>(&w);
+        dst[0] = src[0]; dst[1] = src[1];
+        return w;
+    };
+    auto head_of = [&](int idx) { return idx % shape.head_blocks * shape.fold; };      // first head of the block
+
+    if (warp >= 8) {
+        reg_dec<kRegOther>();
+        if (warp == kProducerWarp) {
+            // =========================== TMA producer ===========================
+            if (lane == 0) {
+                int kv_item = 0;                 // running index into the ring over all items
+                int q_seq = 0;                   // running index of q tiles -> buffer q_seq % kQBufs
+                bool ok = true;
+                auto load_q = [&](const Item& w, int head, int t) {
+                    if (w.blocks[t] == 0 || !ok) return;
+                    const int b = q_seq % kQBufs, use = q_seq / kQBufs;
+                    if (use > 0) ok = mbar_wait(&bar->q_free[b], (use - 1) & 1, abort_flag, 0x110 + b);      // its last product has been made
+                    if (!ok) return;
+                    ++q_seq;
+                    mbar_arrive_expect_tx(&bar->q_full[b], C::kTileBytes);
 #pragma unroll
-    for (int e = 0; e < kE; ++e) { q[e] = Elem<T>::to_f(qp[e]); acc[e] = 0.f; }
-    for (int j = 0; j < n; ++j) {
-        const T* kp = static_cast<const T*>(p.k.ptr) + h * p.k.sh + (s.k0 + j) * p.k.ss + lane * kE;
-        const T* vp = static_cast<const T*>(p.v.ptr) + h * p.v.sh + (s.k0 + j) * p.v.ss + lane * kE;
-        float x = 0.f;
+                    for (int h = 0; h < C::kHalves; ++h)
+                        tma_load_4d(q_smem + b * C::kTileBytes + h * C::kHalfBytes, &maps.q, &bar->q_full[b], h * 64, head, w.q0 + t * shape.tokens, 0);
+                };
+                int round = 0, idx = -1;
+                while (round < n_rounds && (idx = item_of_round(round, n_items)) < 0) ++round;
+                Item w;
+                int head = 0;
+                if (idx >= 0) { w = item_of(idx); head = head_of(idx); load_q(w, head, 0); load_q(w, head, 1); }
+                while (idx >= 0 && ok) {
+                    // one item ahead: its first q tile comes during this item
+                    int round2 = round + 1, idx2 = -1;
+                    while (round2 < n_rounds && (idx2 = item_of_round(round2, n_items)) < 0) ++round2;
+                    Item wn;
+                    int head2 = 0;
+                    if (idx2 >= 0) { wn = item_of(idx2); head2 = head_of(idx2); load_q(wn, head2, 0); }
+                    const int nmax = max(w.blocks[0], w.blocks[1]);
+                    for (int x = 0; x < 2 * nmax && ok; ++x, ++kv_item) {       // x = 2j: K_j, 2j+1: V_j
+                        const int slot = kv_item % kStages;
+                        if (kv_item >= kStages) ok = mbar_wait(&bar->kv_empty[slot], ((kv_item / kStages) - 1) & 1, abort_flag, 0x100);
+                        if (!ok) break;
+                        mbar_arrive_expect_tx(&bar->kv_full[slot], C::kTileBytes);
+                        const CUtensorMap* m = (x & 1) ? &maps.v : &maps.k;
 #pragma unroll
-        for (int e = 0; e < kE; ++e) x = fmaf(q[e], Elem<T>::to_f(kp[e]), x);
+                        for (int h = 0; h < C::kHalves; ++h)
+                            tma_load_4d(kv_smem + slot * C::kTileBytes + h * C::kHalfBytes, m, &bar->kv_full[slot], h * 64, head / rep, w.k0 + (x >> 1) * kBlockN, 0);
+                    }
+                    if (idx2 >= 0) load_q(wn, head2, 1);
+                    idx = idx2; round = round2; w = wn; head = head2;
+                }
+            }
+        } else if (warp == kMmaWarp) {
+            // =========================== MMA issuer ===========================
+            // (bit 13 negates A: the scale's sign, so that the largest product is the largest score)
+            const uint32_t idesc_qk = make_idesc_f16(Elem<T>::kFormat, 0, 0, kBlockM, kBlockN) | (p.scale < 0.f ? 1u << 13 : 0u);
+            constexpr uint32_t idesc_pv = make_idesc_f16(Elem<T>::kFormat, 0, 1, kBlockM, D);
+            const bool leader = elect_one();
+            const uint64_t q_desc = make_smem_desc_sw128(smem_u32(q_smem), 16, 1024), k_desc = make_smem_desc_sw128(smem_u32(kv_smem), 16, 1024);
+            // V is MN-major for its product: 16 keys = 2048 bytes per step, second 64-column box one half-tile further (leading offset)
+            const uint64_t v_desc = make_smem_desc_sw128(smem_u32(kv_smem), C::kHalfBytes, 1024);
+            constexpr uint64_t kTileStep = C::kTileBytes >> 4;
+            // all 512 columns are this CTA's, so they start at 0
+            auto tmem_s = [&](int t) { return static_cast<uint32_t>(t * 128); };
+            auto tmem_o = [&](int t) { return static_cast<uint32_t>(256 + t * 128); };
+            auto commit = [&](uint64_t* b) { if (leader) umma_commit(b); };
+            auto issue_qk = [&](int t, int qbuf, int slot) {
+                const uint64_t a = q_desc + qbuf * kTileStep, bd = k_desc + slot * kTileStep;
+                if (leader)
 #pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, o);
-        x *= p.scale * kLog2e;
-        const float top = fmaxf(m, x), keep = m == -INFINITY ? 0.f : exp2f(m - top), w = exp2f(x - top);
-        l = l * keep + w;
-        m = top;
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        const uint32_t off = ((kk >> 2) * C::kHalfBytes + (kk & 3) * 32) >> 4;
+                        umma_ss(tmem_s(t), a + off, bd + off, idesc_qk, kk > 0 ? 1u : 0u);
+                    }
+            };
+            auto issue_pv = [&](int t, int slot, int steps, bool accumulate) {
+                const uint64_t bd = v_desc + slot * kTileStep;
+                if (leader) {
+                    if (steps == kBlockN / 16) {
 #pragma unroll
-        for (int e = 0; e < kE; ++e) acc[e] = fmaf(w, Elem<T>::to_f(vp[e]), acc[e] * keep);
+                        for (int kk = 0; kk < kBlockN / 16; ++kk)
+                            umma_ts(tmem_o(t), tmem_s(t) + kk * 8, bd + kk * (2048 >> 4), idesc_pv, (accumulate || kk > 0) ? 1u : 0u);
+                    } else {
+                        for (int kk = 0; kk < steps; ++kk)
+                            umma_ts(tmem_o(t), tmem_s(t) + kk * 8, bd + kk * (2048 >> 4), idesc_pv, (accumulate || kk > 0) ? 1u : 0u);
+                    }
+                }
+            };
+            int kv_item = 0, q_seq = 0;
+            int blk[2] = {0, 0};             // running count of score tiles per query tile (barrier phases)
+            bool ok = true;
+            for (int round = 0; round < n_rounds && ok; ++round) {
+                const int idx = item_of_round(round, n_items);
+                if (idx < 0) continue;
+                const Item w = item_of(idx);
+                const int nmax = max(w.blocks[0], w.blocks[1]);
+                if (nmax == 0) continue;
+                int end[2];                  // keys that a row of the tile can see
+#pragma unroll
+                for (int t = 0; t < 2; ++t) end[t] = p.causal ? min(w.keys, w.last + min(w.tokens, (t + 1) * shape.tokens)) : w.keys;
+                int qbuf[2] = {0, 0};
+                const int k0_slot = kv_item % kStages;
+                ok = mbar_wait_warp(&bar->kv_full[k0_slot], (kv_item / kStages) & 1, abort_flag, 0x200);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (w.blocks[t] == 0 || !ok) continue;
+                    qbuf[t] = q_seq % kQBufs;
+                    const int ph = (q_seq / kQBufs) & 1;
+                    ++q_seq;
+                    // S of this tile is free: every PV of the previous item was issued before this point
+                    ok = mbar_wait_warp(&bar->q_full[qbuf[t]], ph, abort_flag, 0x210 + t);
+                    if (!ok) continue;
+                    tc_fence_after();
+                    issue_qk(t, qbuf[t], k0_slot);
+                    commit(&bar->s_full[t]);
+                    if (w.blocks[t] == 1) commit(&bar->q_free[qbuf[t]]);
+                }
+                if (!ok) break;
+                commit(&bar->kv_empty[k0_slot]);
+                for (int j = 0; j < nmax && ok; ++j) {
+                    const int v_item = kv_item + 2 * j + 1, k_item = kv_item + 2 * j + 2;
+                    const int v_slot = v_item % kStages, k_slot = k_item % kStages;
+                    ok = mbar_wait_warp(&bar->kv_full[v_slot], (v_item / kStages) & 1, abort_flag, 0x300);
+                    if (!ok) break;
+                    const int rows = w.keys - j * kBlockN;          // of the sequence in this block of V
+                    if (rows < kBlockN && (rows & 15) != 0) {
+                        // the rest of the last 16 rows that a product may take: cleared
+                        const int n = 16 - (rows & 15);
+                        for (int i = lane; i < n * 8 * C::kHalves; i += 32) {
+                            const int half = i / (n * 8), rem = i - half * (n * 8);
+                            *reinterpret_cast<uint4*>(kv_smem + v_slot * C::kTileBytes + half * C::kHalfBytes + rows * 128 + rem * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                    bool k_ready = false;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        if (j >= w.blocks[t] || !ok) continue;
+                        ok = mbar_wait_warp(&bar->p_ready[t], blk[t] & 1, abort_flag, 0x400 + t);
+                        if (!ok) continue;
+                        ++blk[t];
+                        tc_fence_after();
+                        issue_pv(t, v_slot, min(kBlockN, end[t] - j * kBlockN + 15) >> 4, j > 0);
+                        commit(&bar->o_done[t]);
+                        if (j + 1 < w.blocks[t]) {
+                            if (!k_ready) {
+                                ok = mbar_wait_warp(&bar->kv_full[k_slot], (k_item / kStages) & 1, abort_flag, 0x500);
+                                if (!ok) continue;
+                                tc_fence_after();
+                                k_ready = true;
+                            }
+                            issue_qk(t, qbuf[t], k_slot);
+                            commit(&bar->s_full[t]);
+                            if (j + 2 == w.blocks[t]) commit(&bar->q_free[qbuf[t]]);   // last QK of this tile
+                        }
+                    }
+                    if (!ok) break;
+                    commit(&bar->kv_empty[v_slot]);
+                    if (j + 1 < nmax) commit(&bar->kv_empty[k_slot]);
+                }
+                kv_item += 2 * nmax;
+            }
+            // everything issued so far has to retire before TMEM is released
+            commit(&bar->mma_done);
+            mbar_wait_warp(&bar->mma_done, 0, abort_flag, 0x600);
+        }
+    } else {
+        // =========================== softmax / correction / epilogue ===========================
+        reg_inc<kRegSoftmax>();
+        const int t = warp >> 2;                     // tile of this warpgroup
+        const int r = tid & 127;                     // row inside the tile = TMEM lane
+        const int token = t * shape.tokens + r / shape.fold, head_in = r % shape.fold;
+        const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t s_addr = tmem_base + lane_base + static_cast<uint32_t>(t * 128);
+        const uint32_t o_addr = tmem_base + lane_base + static_cast<uint32_t>(256 + t * 128);
+        // (a scale of zero: the least normal number, which keeps what is masked at -infinity)
+        const float scale_log2 = p.scale == 0.f ? 1.17549435e-38f : fabsf(p.scale) * kLog2e;
+        int g = 0;                                   // running count of score tiles of this query tile
+        bool ok = true;
+
+        for (int round = 0; round < n_rounds && ok; ++round) {
+            const int idx = item_of_round(round, n_items);
+            if (idx < 0) continue;
+            const Item w = item_of(idx);
+            const int n = t ? w.blocks[1] : w.blocks[0];
+            if (t * shape.tokens >= w.tokens) continue;                     // no tokens in this tile
+            const int limit = p.causal ? min(w.keys - 1, w.last + token) : w.keys - 1;      // last visible key of this row
+            const int tile_end = p.causal ? min(w.keys, w.last + min(w.tokens, (t + 1) * shape.tokens)) : w.keys;
+            const int all_see = p.causal ? min(w.keys, w.last + t * shape.tokens + 1) : w.keys;      // keys that every row of the tile sees
+
+            float m_ref = -INFINITY, l_sum = 0.f;
+            for (int j = 0; j < n; ++j, ++g) {
+                ok = mbar_wait_warp(&bar->s_full[t], g & 1, abort_flag, 0x800 + t);
+                if (!ok) break;
+                tc_fence_after();
+                const int k0 = j * kBlockN;
+                const int rest = tile_end - k0;                             // columns that some row sees
+                uint32_t s[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + c * 32, s[c]);
+                tmem_ld_wait();
+                if (k0 + kBlockN > all_see) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (k0 + c * 32 + i > limit) s[c][i] = 0xFF800000u;   // -inf
+                }
+                // row max: 8 independent chains of 3-input max (one thread owns the whole row)
+                float mx8[8];
+#pragma unroll
+                for (int a = 0; a < 8; ++a) mx8[a] = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2)
+                        mx8[(i >> 1) & 7] = fmax3(mx8[(i >> 1) & 7], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
+                const float mx = fmaxf(fmax3(mx8[0], mx8[1], mx8[2]), fmaxf(fmax3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
+                const float m_cand = mx * scale_log2;
+                const bool grow = m_cand > m_ref + kRescale;
+                if (__any_sync(0xFFFFFFFFu, grow)) {
+                    const float m_new = grow ? m_cand : m_ref;
+                    const float alpha = (m_ref == -INFINITY) ? 0.f : fast_exp2(m_ref - m_new);
+                    if (j > 0) {
+                        // all PV products issued so far for this tile must have landed in O
+                        ok = mbar_wait_warp(&bar->o_done[t], (g - 1) & 1, abort_flag, 0x900 + t);
+                        if (!ok) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int c = 0; c < D / 32; ++c) {
+                            uint32_t o[32];
+                            tmem_ld32(o_addr + c * 32, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                            tmem_st32(o_addr + c * 32, o);
+                        }
+                        tmem_st_wait();
+                    }
+                    l_sum *= alpha;
+                    m_ref = m_new;
+                }
+                const float zero = m_ref == -INFINITY ? 0.f : m_ref - kLift;       // no key seen yet: weights of zero
+                float2 rs[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
+                const float2 sc2 = make_float2(scale_log2, scale_log2), nm2 = make_float2(-zero, -zero);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    if (c * 32 >= rest) break;
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        const float2 e = __ffma2_rn(make_float2(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1])), sc2, nm2);
+                        const float2 pp = make_float2(fast_exp2(e.x), fast_exp2(e.y));
+                        rs[(i >> 1) & 3] = __fadd2_rn(rs[(i >> 1) & 3], pp);
+                        pk[i >> 1] = Elem<T>::pack2(pp.x, pp.y);
+                    }
+                    tmem_st16(s_addr + c * 16, pk);
+                }
+                l_sum += ((rs[0].x + rs[0].y) + (rs[1].x + rs[1].y)) + ((rs[2].x + rs[2].y) + (rs[3].x + rs[3].y));
+                tmem_st_wait();
+                tc_fence_before();
+                mbar_arrive(&bar->p_ready[t]);
+            }
+            if (!ok) break;
+
+            // ---- epilogue of this item: O / l -> global, LSE ----
+            if (n > 0) {
+                ok = mbar_wait_warp(&bar->o_done[t], (g - 1) & 1, abort_flag, 0xA00 + t);
+                if (!ok) break;
+                tc_fence_after();
+            }
+            const bool row_live = token < w.tokens;
+            const float inv_l = l_sum == 0.f ? 0.f : 1.0f / l_sum;          // (a row that sees no key)
+            const int hq = head_of(idx) + head_in;
+            T* orow = static_cast<T*>(p.o.ptr) + hq * p.o.sh + static_cast<long long>(w.q0 + token) * p.o.ss;
+            const bool o32 = (reinterpret_cast<uintptr_t>(orow) & 31) == 0;     // every segment offset below is a multiple of 32 bytes
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];                          // (a tile without keys reads what stands there, and writes zeros)
+                tmem_ld32(o_addr + c * 32, o);
+                tmem_ld_wait();
+                if (row_live) {
+#pragma unroll
+                    for (int v = 0; v < 2; ++v) {
+                        uint32_t w8[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            w8[e] = l_sum == 0.f ? 0u : Elem<T>::pack2(__uint_as_float(o[16 * v + 2 * e]) * inv_l, __uint_as_float(o[16 * v + 2 * e + 1]) * inv_l);
+                        if (o32) {
+                            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                                         ::"l"(orow + c * 32 + v * 16), "r"(w8[0]), "r"(w8[1]), "r"(w8[2]), "r"(w8[3]), "r"(w8[4]), "r"(w8[5]),
+                                           "r"(w8[6]), "r"(w8[7]) : "memory");
+                        } else {                     // the interface promises 16-byte alignment only
+                            uint4* o4 = reinterpret_cast<uint4*>(orow + c * 32 + v * 16);
+                            o4[0] = make_uint4(w8[0], w8[1], w8[2], w8[3]);
+                            o4[1] = make_uint4(w8[4], w8[5], w8[6], w8[7]);
+                        }
+                    }
+                }
+            }
+            // O has been read out: the next item's first PV (issued only after this thread's next p_ready arrival) may overwrite it
+            tc_fence_before();
+            if (p.lse != nullptr && row_live)
+                p.lse[static_cast<long long>(hq) * p.total_q + w.q0 + token] = l_sum == 0.f ? -INFINITY : (m_ref - kLift + fast_log2(l_sum)) * kLn2;
+        }
     }
-    T* op = static_cast<T*>(p.o.ptr) + hq * p.o.sh + token * p.o.ss + lane * kE;
-#pragma unroll
-    for (int e = 0; e < kE; ++e) op[e] = Elem<T>::from_f(l == 0.f ? 0.f : acc[e] / l);
-    if (p.lse && lane == 0) p.lse[static_cast<long long>(hq) * p.total_q + token] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+
+    // ---- teardown ----
+    tc_fence_before();
+    __syncthreads();
+    abort_linger(&bar->abort_flag);
+    if (warp == kMmaWarp) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, 512);
+    }
+}
+
+// ---- host side ----
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn() {
+    static EncodeTiledFn fn = []() -> EncodeTiledFn {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult qres;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &qres) != cudaSuccess || qres != cudaDriverEntryPointSuccess) return nullptr;
+        return reinterpret_cast<EncodeTiledFn>(ptr);
+    }();
+    return fn;
+}
+
+// [tokens, H, D] view -> 4-D map (D, H, tokens, 1), box [64 columns][heads][tokens], 128-byte swizzle
+int make_map(CUtensorMap* m, int dtype, const View4& v, int tokens, int H, int D, int box_heads, int box_tokens) {
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) return set_detail(VB200_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(H), static_cast<cuuint64_t>(tokens), 1};
+    cuuint64_t strides[3] = {static_cast<cuuint64_t>(v.sh) * 2, static_cast<cuuint64_t>(v.ss) * 2, 16};
+    for (int i = 0; i < 2; ++i) if (strides[i] == 0) strides[i] = 16;          // (of extent 1: any legal stride)
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_tokens), 1};
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    const CUresult r = enc(m, dtype == VB200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, v.ptr, dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        static thread_local char buf[96];
+        snprintf(buf, sizeof(buf), "cuTensorMapEncodeTiled (packed attention) failed with CUresult %d", static_cast<int>(r));
+        return set_detail(VB200_ERR_CUDA, buf);
+    }
+    return VB200_OK;
+}
+
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+struct Carve {
+    size_t items, first, total;            // offsets
+};
+Carve carve(int batch, const Shape& s) {
+    Carve c;
+    c.items = 256;
+    c.first = c.items + up256(sizeof(Item) * static_cast<size_t>(s.max_items));
+    c.total = c.first + up256(sizeof(int) * (static_cast<size_t>(batch) + 1));
+    return c;
 }
 
 template <typename T, int D>
 int launch_t(cudaStream_t s, const PackedParams& p) {
-    prefill_packed_kernel<T, D><<<dim3((p.total_q + kWarps - 1) / kWarps, p.Hq), kWarps * 32, 0, s>>>(p);
+    static thread_local bool configured[64] = {};      // per device ordinal: the attribute belongs to the device's context
+    int dev = 0;
+    VB200_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64) return set_detail(VB200_ERR_NO_DEVICE, "device ordinal out of range");
+    if (!configured[dev]) {
+        VB200_CUDA_TRY(cudaFuncSetAttribute(prefill_packed_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmemBytes));
+        configured[dev] = true;
+    }
+    const Shape shape = shape_of(p.batch, p.Hq, p.Hkv, p.total_q);
+    const Carve c = carve(p.batch, shape);
+    char* ws = static_cast<char*>(p.workspace);
+    Plan* plan = reinterpret_cast<Plan*>(ws);
+    Item* items = reinterpret_cast<Item*>(ws + c.items);
+    TmaMaps maps;
+    if (int rc = make_map(&maps.q, p.dtype, p.q, p.total_q, p.Hq, D, shape.fold, shape.tokens)) return rc;
+    // no keys at all: no block is loaded, any map will do
+    const View4 k = p.total_k > 0 ? p.k : p.q, v = p.total_k > 0 ? p.v : p.q;
+    const int n_k = p.total_k > 0 ? p.total_k : p.total_q, h_k = p.total_k > 0 ? p.Hkv : p.Hq;
+    if (int rc = make_map(&maps.k, p.dtype, k, n_k, h_k, D, 1, kBlockN)) return rc;
+    if (int rc = make_map(&maps.v, p.dtype, v, n_k, h_k, D, 1, kBlockN)) return rc;
+    packed_plan_kernel<<<1, kPlanThreads, 0, s>>>(p, shape.tokens, shape.max_items, plan, items, reinterpret_cast<int*>(ws + c.first));
     note_launch();
     VB200_CUDA_TRY(cudaPeekAtLastError());
+    const int64_t most = static_cast<int64_t>(shape.max_items) * shape.head_blocks;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(most, device_sm_count())));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Cfg<D>::kSmemBytes;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    profile_mark_begin(s);
+    VB200_CUDA_TRY(cudaLaunchKernelEx(&cfg, prefill_packed_kernel<T, D>, maps, p, shape, static_cast<const Plan*>(plan), static_cast<const Item*>(items)));
+    profile_mark_end(s);
+    note_launch();
     return VB200_OK;
 }
 
 }  // namespace
 
-size_t prefill_packed_workspace(int, int, int, int) { return 256; }
+size_t prefill_packed_workspace(int batch, int Hq, int Hkv, int total_q) { return carve(batch, shape_of(batch, Hq, Hkv, total_q)).total; }
 
 int launch_prefill_packed(cudaStream_t s, const PackedParams& p) {
     if (p.dtype == VB200_BF16) return p.D == 128 ? launch_t<__nv_bfloat16, 128>(s, p) : launch_t<__nv_bfloat16, 64>(s, p);
