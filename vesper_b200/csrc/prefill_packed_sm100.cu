@@ -5,14 +5,17 @@
 //
 // A tile is 128 rows: 128 / F tokens of one sequence by F heads of one key head's group (F: the power of two of the group, at most 16), row = token * F +
 // head, as one TMA box of q brings them.  Short sequences fill a tile with heads instead of padding, and the rows of a tile see nearly the same keys.  A work
-// item is two tiles of neighbouring tokens that read the same blocks of 128 keys.  The lengths are on the device: a first kernel lists the items with the
+// item is two tiles of neighbouring tokens that read the same blocks of keys.  The lengths are on the device: a first kernel lists the items with the
 // longest first, then persistent CTAs, one per SM, take them in snake order.
 //   warps 0-3    softmax and epilogue of tile 0, a row per thread (TMEM lane)
 //   warps 4-7    the same for tile 1
 //   warp  8      TMA: q tiles (3 buffers, so that the next item's come while this one computes) and the ring of key and value blocks
-//   warp  9      tcgen05.mma issuer, TMEM owner
-// TMEM (512 columns): S0 [0,128) S1 [128,256) O0 [256,256+D) O1 [384,384+D); the weights (16 bits, two to a column) overwrite the first 64 columns of their S.
-// The last block of a tile takes only the columns (by 32) and the rows of V (by 16) that a row of it can see.  The rows of V behind the sequence in its last
+//   warps 9, 10  tcgen05.mma issuers of tile 0 and of tile 1; warp 9 owns the TMEM
+// TMEM (512 columns): per tile the scores S of a block, its weights (16 bits, two to a column) beside them, and O.  The weights do not overwrite the scores, so
+// that the next block's Q K^T is made while this block's weights are computed: with head_dim 128 a block is 80 keys (2 x (80 + 40 + 128) columns), with 64 it
+// is 128 keys (2 x (128 + 64 + 64)).  (Blocks of 128 keys whose weights overwrote their scores, head_dim 128: 518 us for 24 prompts of 16-4057 tokens, tensor
+// pipe busy 49 %, the softmax and the products of a tile waiting for each other.)
+// The last block of a tile takes only the columns and rows of V, by 16, that a row of it can see.  The rows of V behind the sequence in its last
 // 16 are another sequence's, or nobody's: they are cleared in shared memory, since a weight of zero does not silence a NaN.
 // Every wait is bounded (mbar_wait); on expiry the CTA drains and returns with the status word set.
 #include "hybrid.cuh"
@@ -20,13 +23,13 @@
 
 #include <algorithm>
 #include <cstdio>
+#include <type_traits>
 
 namespace vb200 {
 
 namespace {
 
-constexpr int kBlockM = 128, kBlockN = 128;
-constexpr int kStages = 4;                 // key / value slots
+constexpr int kBlockM = 128;
 constexpr int kQBufs = 3;
 constexpr int kProducerWarp = 8, kMmaWarp = 9;
 constexpr int kThreads = 384;              // three warpgroups: registers are moved by warpgroups
@@ -40,7 +43,7 @@ static_assert(kRegSoftmax * 256 + kRegOther * 128 <= 168 * 384, "register budget
 // sees is `last` + i (causal).
 struct alignas(16) Item {
     int q0, tokens, k0, keys;
-    int last, blocks[2], pad;              // key blocks of each tile
+    int last, end[2], pad;                 // keys that some row of each tile sees; -1: the tile has no tokens
 };
 
 struct Plan {                              // workspace: the header, the items, the first item of each sequence
@@ -63,10 +66,11 @@ Shape shape_of(int batch, int Hq, int Hkv, int total_q) {
     return s;
 }
 
-// ---- the list of items, by descending number of key blocks ----
+// ---- the list of items, by descending number of keys ----
 constexpr int kPlanThreads = 1024, kBins = 1024;
 
-__device__ __forceinline__ int bin_of(int blocks) {      // longest first
+__device__ __forceinline__ int bin_of(int keys) {        // longest first
+    const int blocks = (max(keys, 0) + 63) / 64;
     return kBins - 1 - (blocks < 512 ? blocks : 512 + min(511, (blocks - 512) >> 4));
 }
 
@@ -140,14 +144,14 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedParams 
         w.pad = 0;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const int end = p.causal ? min(s.nk, w.last + min(w.tokens, (t + 1) * tile_tokens)) : s.nk;
-            w.blocks[t] = w.tokens > t * tile_tokens && end > 0 ? (end + kBlockN - 1) / kBlockN : 0;
+            const int end = p.causal ? max(0, min(s.nk, w.last + min(w.tokens, (t + 1) * tile_tokens))) : s.nk;
+            w.end[t] = w.tokens > t * tile_tokens ? end : -1;
         }
         return w;
     };
     for (int idx = tid; idx < n; idx += kPlanThreads) {
         const Item w = item_at(idx);
-        atomicAdd(&hist[bin_of(max(w.blocks[0], w.blocks[1]))], 1);
+        atomicAdd(&hist[bin_of(max(w.end[0], w.end[1]))], 1);
     }
     __syncthreads();
     const int count = hist[tid];
@@ -156,15 +160,15 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedParams 
     __syncthreads();
     for (int idx = tid; idx < n; idx += kPlanThreads) {  // (the order within a bin is free: results do not depend on it)
         const Item w = item_at(idx);
-        items[atomicAdd(&hist[bin_of(max(w.blocks[0], w.blocks[1]))], 1)] = w;
+        items[atomicAdd(&hist[bin_of(max(w.end[0], w.end[1]))], 1)] = w;
     }
 }
 
 // ---- the attention kernel ----
 struct __align__(8) Barriers {
     uint64_t q_full[kQBufs], q_free[kQBufs];
-    uint64_t kv_full[kStages], kv_empty[kStages];
-    uint64_t s_full[2], p_ready[2], o_done[2];
+    uint64_t kv_full[8], kv_empty[8];
+    uint64_t s_full[2], s_free[2], p_ready[2], o_done[2];
     uint64_t mma_done;
     uint32_t tmem_base;
     int abort_flag;
@@ -176,11 +180,20 @@ struct TmaMaps {
 
 template <int D>
 struct Cfg {
+    static constexpr int kN = D == 128 ? 80 : 112;               // keys of a block
+    static constexpr int kStages = D == 128 ? 6 : 8;             // key / value slots
+    static constexpr int kOnFma = 1;
     static constexpr int kHalves = D / 64;                       // 64-column (128-byte) boxes per row
-    static constexpr int kHalfBytes = 128 * 128;                 // one [128 rows][64 cols] 16-bit box
-    static constexpr int kTileBytes = kHalves * kHalfBytes;
-    static constexpr int kSmemBytes = (kQBufs + kStages) * kTileBytes + 1024 /*alignment slack*/ + 256 /*Barriers*/;
+    static constexpr int kQHalf = kBlockM * 128, kQTile = kHalves * kQHalf;
+    static constexpr int kKvHalf = kN * 128, kKvTile = kHalves * kKvHalf;
+    static constexpr int kTile = kN + kN / 2;                    // TMEM columns of a tile's scores and weights
+    static constexpr int kS(int t) { return t * (D == 128 ? 128 : kTile); }
+    static constexpr int kP(int t) { return kS(t) + kN; }
+    static constexpr int kO(int t) { return 512 - (2 - t) * D; }
+    static constexpr int kSmemBytes = kQBufs * kQTile + kStages * kKvTile + 1024 /*alignment slack*/ + 256 /*Barriers*/;
+    static_assert(kP(1) + kN / 2 <= kO(0) && kStages <= 8 && kSmemBytes <= 227 * 1024, "layout");
 };
+__device__ __forceinline__ int blocks_of(int end, int n) { return end > 0 ? (end + n - 1) / n : 0; }
 static_assert(sizeof(Barriers) <= 256, "room for the barriers");
 
 // Round r gives CTA c item r * G + c (even r) or r * G + G - 1 - c (odd r), which evens out the sums.  -1: none.
@@ -193,14 +206,44 @@ __device__ __forceinline__ int item_of_round(int round, int n_items) {
 template <int N> __device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
+// whether the phase is over, without waiting
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return ok != 0;
+}
+
+// 2^x on the FMA pipe for two numbers: x = n + f with n the nearest whole number (Cody-Waite), a polynomial of degree 4 for 2^f on [-1/2, 1/2] (fitted for
+// the least relative error, 2.6e-6), and n added to the exponent.  For x above -126; what is below gives 2^-126, so masked scores do not come here.
+__device__ __forceinline__ float2 exp2_fma(float2 x) {
+    float a, b;
+    asm("max.NaN.f32 %0, %1, 0fC2FC0000;" : "=f"(a) : "f"(x.x));             // -126; a NaN stays one
+    asm("max.NaN.f32 %0, %1, 0fC2FC0000;" : "=f"(b) : "f"(x.y));
+    x = make_float2(a, b);
+    constexpr float kMagic = 12582912.0f;                                    // 1.5 * 2^23: the sum's last bits are n
+    const float2 z = __fadd2_rn(x, make_float2(kMagic, kMagic));
+    const float2 n = __fadd2_rn(z, make_float2(-kMagic, -kMagic));
+    const float2 f = __ffma2_rn(n, make_float2(-1.0f, -1.0f), x);
+    float2 y = make_float2(0.0095701f, 0.0095701f);
+    y = __ffma2_rn(y, f, make_float2(0.05591786f, 0.05591786f));
+    y = __ffma2_rn(y, f, make_float2(0.24024745f, 0.24024745f));
+    y = __ffma2_rn(y, f, make_float2(0.69312181f, 0.69312181f));
+    y = __ffma2_rn(y, f, make_float2(0.99999926f, 0.99999926f));
+    return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(z.x) << 23)), __int_as_float(__float_as_int(y.y) + (__float_as_int(z.y) << 23)));
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __grid_constant__ TmaMaps maps, PackedParams p, Shape shape, const Plan* plan, const Item* items) {
     using C = Cfg<D>;
     extern __shared__ unsigned char smem_dyn[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));      // 128B-swizzled tiles
     unsigned char* q_smem = smem;                                   // kQBufs tiles
-    unsigned char* kv_smem = smem + kQBufs * C::kTileBytes;         // kStages tiles
-    Barriers* bar = reinterpret_cast<Barriers*>(smem + (kQBufs + kStages) * C::kTileBytes);
+    unsigned char* kv_smem = smem + kQBufs * C::kQTile;             // C::kStages tiles
+    Barriers* bar = reinterpret_cast<Barriers*>(kv_smem + C::kStages * C::kKvTile);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -208,9 +251,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __gri
     if (warp == kMmaWarp) {
         if (lane == 0) {
             for (int b = 0; b < kQBufs; ++b) { mbar_init(&bar->q_full[b], 1); mbar_init(&bar->q_free[b], 1); }
-            for (int t = 0; t < 2; ++t) { mbar_init(&bar->s_full[t], 1); mbar_init(&bar->p_ready[t], kBlockM); mbar_init(&bar->o_done[t], 1); }
-            for (int s = 0; s < kStages; ++s) { mbar_init(&bar->kv_full[s], 1); mbar_init(&bar->kv_empty[s], 1); }
-            mbar_init(&bar->mma_done, 1);
+            for (int t = 0; t < 2; ++t) { mbar_init(&bar->s_full[t], 1); mbar_init(&bar->s_free[t], 4); mbar_init(&bar->p_ready[t], 4); mbar_init(&bar->o_done[t], 1); }
+            for (int s = 0; s < C::kStages; ++s) { mbar_init(&bar->kv_full[s], 1); mbar_init(&bar->kv_empty[s], 2); }
+            mbar_init(&bar->mma_done, 2);
             bar->abort_flag = 0;
             mbar_fence_init();
         }
@@ -247,15 +290,15 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __gri
                 int q_seq = 0;                   // running index of q tiles -> buffer q_seq % kQBufs
                 bool ok = true;
                 auto load_q = [&](const Item& w, int head, int t) {
-                    if (w.blocks[t] == 0 || !ok) return;
+                    if (w.end[t] <= 0 || !ok) return;
                     const int b = q_seq % kQBufs, use = q_seq / kQBufs;
                     if (use > 0) ok = mbar_wait(&bar->q_free[b], (use - 1) & 1, abort_flag, 0x110 + b);      // its last product has been made
                     if (!ok) return;
                     ++q_seq;
-                    mbar_arrive_expect_tx(&bar->q_full[b], C::kTileBytes);
+                    mbar_arrive_expect_tx(&bar->q_full[b], C::kQTile);
 #pragma unroll
                     for (int h = 0; h < C::kHalves; ++h)
-                        tma_load_4d(q_smem + b * C::kTileBytes + h * C::kHalfBytes, &maps.q, &bar->q_full[b], h * 64, head, w.q0 + t * shape.tokens, 0);
+                        tma_load_4d(q_smem + b * C::kQTile + h * C::kQHalf, &maps.q, &bar->q_full[b], h * 64, head, w.q0 + t * shape.tokens, 0);
                 };
                 int round = 0, idx = -1;
                 while (round < n_rounds && (idx = item_of_round(round, n_items)) < 0) ++round;
@@ -269,135 +312,123 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __gri
                     Item wn;
                     int head2 = 0;
                     if (idx2 >= 0) { wn = item_of(idx2); head2 = head_of(idx2); load_q(wn, head2, 0); }
-                    const int nmax = max(w.blocks[0], w.blocks[1]);
-                    for (int x = 0; x < 2 * nmax && ok; ++x, ++kv_item) {       // x = 2j: K_j, 2j+1: V_j
-                        const int slot = kv_item % kStages;
-                        if (kv_item >= kStages) ok = mbar_wait(&bar->kv_empty[slot], ((kv_item / kStages) - 1) & 1, abort_flag, 0x100);
+                    const int nmax = blocks_of(max(w.end[0], w.end[1]), C::kN);
+                    // in the order in which the products take them: K0, then K(j+1), V(j)
+                    for (int x = 0; x < 2 * nmax && ok; ++x, ++kv_item) {
+                        const int slot = kv_item % C::kStages;
+                        if (kv_item >= C::kStages) ok = mbar_wait(&bar->kv_empty[slot], ((kv_item / C::kStages) - 1) & 1, abort_flag, 0x100);
                         if (!ok) break;
-                        mbar_arrive_expect_tx(&bar->kv_full[slot], C::kTileBytes);
-                        const CUtensorMap* m = (x & 1) ? &maps.v : &maps.k;
+                        const bool value = x == 2 * nmax - 1 || (x > 0 && (x & 1) == 0);
+                        const int block = x == 0 ? 0 : value ? (x - 1) / 2 : (x + 1) / 2;
+                        mbar_arrive_expect_tx(&bar->kv_full[slot], C::kKvTile);
+                        const CUtensorMap* m = value ? &maps.v : &maps.k;
 #pragma unroll
                         for (int h = 0; h < C::kHalves; ++h)
-                            tma_load_4d(kv_smem + slot * C::kTileBytes + h * C::kHalfBytes, m, &bar->kv_full[slot], h * 64, head / rep, w.k0 + (x >> 1) * kBlockN, 0);
+                            tma_load_4d(kv_smem + slot * C::kKvTile + h * C::kKvHalf, m, &bar->kv_full[slot], h * 64, head / rep, w.k0 + block * C::kN, 0);
                     }
                     if (idx2 >= 0) load_q(wn, head2, 1);
                     idx = idx2; round = round2; w = wn; head = head2;
                 }
             }
-        } else if (warp == kMmaWarp) {
-            // =========================== MMA issuer ===========================
-            // (bit 13 negates A: the scale's sign, so that the largest product is the largest score)
-            const uint32_t idesc_qk = make_idesc_f16(Elem<T>::kFormat, 0, 0, kBlockM, kBlockN) | (p.scale < 0.f ? 1u << 13 : 0u);
-            constexpr uint32_t idesc_pv = make_idesc_f16(Elem<T>::kFormat, 0, 1, kBlockM, D);
-            const bool leader = elect_one();
-            const uint64_t q_desc = make_smem_desc_sw128(smem_u32(q_smem), 16, 1024), k_desc = make_smem_desc_sw128(smem_u32(kv_smem), 16, 1024);
-            // V is MN-major for its product: 16 keys = 2048 bytes per step, second 64-column box one half-tile further (leading offset)
-            const uint64_t v_desc = make_smem_desc_sw128(smem_u32(kv_smem), C::kHalfBytes, 1024);
-            constexpr uint64_t kTileStep = C::kTileBytes >> 4;
-            // all 512 columns are this CTA's, so they start at 0
-            auto tmem_s = [&](int t) { return static_cast<uint32_t>(t * 128); };
-            auto tmem_o = [&](int t) { return static_cast<uint32_t>(256 + t * 128); };
-            auto commit = [&](uint64_t* b) { if (leader) umma_commit(b); };
-            auto issue_qk = [&](int t, int qbuf, int slot) {
-                const uint64_t a = q_desc + qbuf * kTileStep, bd = k_desc + slot * kTileStep;
-                if (leader)
+        } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
+            // =========================== MMA issuers, one for each tile ===========================
+            // One elected thread walks the items, waits and issues: in code that the whole warp runs, a wait costs 100 to 200 cycles and a product 50.  What
+            // such a thread has to do for two tiles takes longer than their softmax, so each tile has one.  (8192 keys and queries, 32 heads, a whole
+            // warp for both tiles: 915 TFLOP/s, a thread for both: 1132.)
+            const int t = warp - kMmaWarp;
+            if (elect_one()) {
+                // (bit 13 negates A: the scale's sign, so that the largest product is the largest score)
+                const uint32_t idesc_qk = make_idesc_f16(Elem<T>::kFormat, 0, 0, kBlockM, C::kN) | (p.scale < 0.f ? 1u << 13 : 0u);
+                constexpr uint32_t idesc_pv = make_idesc_f16(Elem<T>::kFormat, 0, 1, kBlockM, D);
+                // V is MN-major for its product: 16 keys = 2048 bytes per step, second 64-column box one half-tile further (leading offset)
+                const uint64_t q_desc = make_smem_desc_sw128(smem_u32(q_smem), 16, 1024), k_desc = make_smem_desc_sw128(smem_u32(kv_smem), 16, 1024);
+                const uint64_t v_desc = make_smem_desc_sw128(smem_u32(kv_smem), C::kKvHalf, 1024);
+                // all 512 columns are this CTA's, so they start at 0
+                const uint32_t s_tmem = t ? C::kS(1) : C::kS(0), p_tmem = t ? C::kP(1) : C::kP(0), o_tmem = t ? C::kO(1) : C::kO(0);
+                auto issue_pv = [&](int slot, int steps, bool accumulate) {
+                    const uint64_t bd = v_desc + slot * (C::kKvTile >> 4);
+                    if (steps == C::kN / 16) {
 #pragma unroll
-                    for (int kk = 0; kk < D / 16; ++kk) {
-                        const uint32_t off = ((kk >> 2) * C::kHalfBytes + (kk & 3) * 32) >> 4;
-                        umma_ss(tmem_s(t), a + off, bd + off, idesc_qk, kk > 0 ? 1u : 0u);
-                    }
-            };
-            auto issue_pv = [&](int t, int slot, int steps, bool accumulate) {
-                const uint64_t bd = v_desc + slot * kTileStep;
-                if (leader) {
-                    if (steps == kBlockN / 16) {
-#pragma unroll
-                        for (int kk = 0; kk < kBlockN / 16; ++kk)
-                            umma_ts(tmem_o(t), tmem_s(t) + kk * 8, bd + kk * (2048 >> 4), idesc_pv, (accumulate || kk > 0) ? 1u : 0u);
+                        for (int kk = 0; kk < C::kN / 16; ++kk)
+                            umma_ts(o_tmem, p_tmem + kk * 8, bd + kk * (2048 >> 4), idesc_pv, (accumulate || kk > 0) ? 1u : 0u);
                     } else {
                         for (int kk = 0; kk < steps; ++kk)
-                            umma_ts(tmem_o(t), tmem_s(t) + kk * 8, bd + kk * (2048 >> 4), idesc_pv, (accumulate || kk > 0) ? 1u : 0u);
+                            umma_ts(o_tmem, p_tmem + kk * 8, bd + kk * (2048 >> 4), idesc_pv, (accumulate || kk > 0) ? 1u : 0u);
                     }
-                }
-            };
-            int kv_item = 0, q_seq = 0;
-            int blk[2] = {0, 0};             // running count of score tiles per query tile (barrier phases)
-            bool ok = true;
-            for (int round = 0; round < n_rounds && ok; ++round) {
-                const int idx = item_of_round(round, n_items);
-                if (idx < 0) continue;
-                const Item w = item_of(idx);
-                const int nmax = max(w.blocks[0], w.blocks[1]);
-                if (nmax == 0) continue;
-                int end[2];                  // keys that a row of the tile can see
-#pragma unroll
-                for (int t = 0; t < 2; ++t) end[t] = p.causal ? min(w.keys, w.last + min(w.tokens, (t + 1) * shape.tokens)) : w.keys;
-                int qbuf[2] = {0, 0};
-                const int k0_slot = kv_item % kStages;
-                ok = mbar_wait_warp(&bar->kv_full[k0_slot], (kv_item / kStages) & 1, abort_flag, 0x200);
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    if (w.blocks[t] == 0 || !ok) continue;
-                    qbuf[t] = q_seq % kQBufs;
-                    const int ph = (q_seq / kQBufs) & 1;
-                    ++q_seq;
-                    // S of this tile is free: every PV of the previous item was issued before this point
-                    ok = mbar_wait_warp(&bar->q_full[qbuf[t]], ph, abort_flag, 0x210 + t);
-                    if (!ok) continue;
-                    tc_fence_after();
-                    issue_qk(t, qbuf[t], k0_slot);
-                    commit(&bar->s_full[t]);
-                    if (w.blocks[t] == 1) commit(&bar->q_free[qbuf[t]]);
-                }
-                if (!ok) break;
-                commit(&bar->kv_empty[k0_slot]);
-                for (int j = 0; j < nmax && ok; ++j) {
-                    const int v_item = kv_item + 2 * j + 1, k_item = kv_item + 2 * j + 2;
-                    const int v_slot = v_item % kStages, k_slot = k_item % kStages;
-                    ok = mbar_wait_warp(&bar->kv_full[v_slot], (v_item / kStages) & 1, abort_flag, 0x300);
-                    if (!ok) break;
-                    const int rows = w.keys - j * kBlockN;          // of the sequence in this block of V
-                    if (rows < kBlockN && (rows & 15) != 0) {
-                        // the rest of the last 16 rows that a product may take: cleared
-                        const int n = 16 - (rows & 15);
-                        for (int i = lane; i < n * 8 * C::kHalves; i += 32) {
-                            const int half = i / (n * 8), rem = i - half * (n * 8);
-                            *reinterpret_cast<uint4*>(kv_smem + v_slot * C::kTileBytes + half * C::kHalfBytes + rows * 128 + rem * 16) = make_uint4(0, 0, 0, 0);
-                        }
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                    }
-                    bool k_ready = false;
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        if (j >= w.blocks[t] || !ok) continue;
-                        ok = mbar_wait_warp(&bar->p_ready[t], blk[t] & 1, abort_flag, 0x400 + t);
-                        if (!ok) continue;
-                        ++blk[t];
-                        tc_fence_after();
-                        issue_pv(t, v_slot, min(kBlockN, end[t] - j * kBlockN + 15) >> 4, j > 0);
-                        commit(&bar->o_done[t]);
-                        if (j + 1 < w.blocks[t]) {
-                            if (!k_ready) {
-                                ok = mbar_wait_warp(&bar->kv_full[k_slot], (k_item / kStages) & 1, abort_flag, 0x500);
-                                if (!ok) continue;
+                };
+                int slot = 0, kv_phase = 0, qb = 0, q_phase = 0;
+                auto next_slot = [&]() { if (++slot == C::kStages) { slot = 0; kv_phase ^= 1; } };
+                uint32_t s_phase = 1, p_phase = 0;               // (the first wait for free scores passes: none have been made)
+                bool ok = true;
+                for (int round = 0; round < n_rounds && ok; ++round) {
+                    const int idx = item_of_round(round, n_items);
+                    if (idx < 0) continue;
+                    const Item w = item_of(idx);
+                    const int end = t ? w.end[1] : w.end[0], n = blocks_of(end, C::kN), nmax = blocks_of(max(w.end[0], w.end[1]), C::kN);
+                    // the q tiles of an item: tile 0's buffer, if it has one, then tile 1's
+                    const bool q0 = w.end[0] > 0, q1 = w.end[1] > 0;
+                    auto next_q = [&]() { if (++qb == kQBufs) { qb = 0; q_phase ^= 1; } };
+                    if (t == 1 && q0) next_q();
+                    const int qbuf = qb;
+                    const uint64_t qd = q_desc + qbuf * (C::kQTile >> 4);
+                    if (n > 0) ok = mbar_wait(&bar->q_full[qbuf], q_phase, abort_flag, 0x210 + t);
+                    if (t == 0 ? q0 : q1) next_q();
+                    if (t == 0 && q1) next_q();
+                    // j = -1: the first scores; then the scores of block j + 1 and the weighted values of block j
+                    for (int j = -1; j < nmax && ok; ++j) {
+                        if (j + 1 < nmax) {
+                            ok = mbar_wait(&bar->kv_full[slot], kv_phase, abort_flag, 0x200);
+                            if (!ok) break;
+                            if (j + 1 < n) {
+                                // the scores before these, of this item or the one before it, have been read
+                                ok = mbar_wait(&bar->s_free[t], s_phase, abort_flag, 0x220 + t);
+                                if (!ok) break;
+                                s_phase ^= 1;
                                 tc_fence_after();
-                                k_ready = true;
+                                const uint64_t bd = k_desc + slot * (C::kKvTile >> 4);
+#pragma unroll
+                                for (int kk = 0; kk < D / 16; ++kk)
+                                    umma_ss(s_tmem, qd + (((kk >> 2) * C::kQHalf + (kk & 3) * 32) >> 4), bd + (((kk >> 2) * C::kKvHalf + (kk & 3) * 32) >> 4), idesc_qk, kk > 0 ? 1u : 0u);
+                                umma_commit(&bar->s_full[t]);
+                                umma_commit(&bar->kv_empty[slot]);
+                                if (j + 2 == n) umma_commit(&bar->q_free[qbuf]);      // the last product of this q tile
+                            } else {
+                                mbar_arrive(&bar->kv_empty[slot]);                    // a block for the other tile
                             }
-                            issue_qk(t, qbuf[t], k_slot);
-                            commit(&bar->s_full[t]);
-                            if (j + 2 == w.blocks[t]) commit(&bar->q_free[qbuf[t]]);   // last QK of this tile
+                            next_slot();
                         }
+                        if (j < 0) continue;
+                        ok = mbar_wait(&bar->kv_full[slot], kv_phase, abort_flag, 0x300);
+                        if (!ok) break;
+                        if (j < n) {
+                            const int rows = w.keys - j * C::kN;        // of the sequence in this block of V
+                            if (rows < C::kN && (rows & 15) != 0) {
+                                // the rest of the last 16 rows that a product may take: cleared (by both issuers, each before its own product)
+                                const int m = 16 - (rows & 15);
+#pragma unroll
+                                for (int half = 0; half < C::kHalves; ++half)
+                                    for (int i = 0; i < m * 8; ++i)
+                                        *reinterpret_cast<uint4*>(kv_smem + slot * C::kKvTile + half * C::kKvHalf + rows * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+                                fence_proxy_async_smem();
+                            }
+                            ok = mbar_wait(&bar->p_ready[t], p_phase, abort_flag, 0x400 + t);
+                            if (!ok) break;
+                            p_phase ^= 1;
+                            tc_fence_after();
+                            issue_pv(slot, min(C::kN, end - j * C::kN + 15) >> 4, j > 0);
+                            umma_commit(&bar->o_done[t]);
+                            umma_commit(&bar->kv_empty[slot]);
+                        } else {
+                            mbar_arrive(&bar->kv_empty[slot]);
+                        }
+                        next_slot();
                     }
-                    if (!ok) break;
-                    commit(&bar->kv_empty[v_slot]);
-                    if (j + 1 < nmax) commit(&bar->kv_empty[k_slot]);
                 }
-                kv_item += 2 * nmax;
+                // everything issued so far has to retire before TMEM is released
+                umma_commit(&bar->mma_done);
+                mbar_wait(&bar->mma_done, 0, abort_flag, 0x600);
             }
-            // everything issued so far has to retire before TMEM is released
-            commit(&bar->mma_done);
-            mbar_wait_warp(&bar->mma_done, 0, abort_flag, 0x600);
+            __syncwarp();
         }
     } else {
         // =========================== softmax / correction / epilogue ===========================
@@ -406,8 +437,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __gri
         const int r = tid & 127;                     // row inside the tile = TMEM lane
         const int token = t * shape.tokens + r / shape.fold, head_in = r % shape.fold;
         const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t s_addr = tmem_base + lane_base + static_cast<uint32_t>(t * 128);
-        const uint32_t o_addr = tmem_base + lane_base + static_cast<uint32_t>(256 + t * 128);
+        const uint32_t s_addr = tmem_base + lane_base + (t ? C::kS(1) : C::kS(0));
+        const uint32_t p_addr = tmem_base + lane_base + (t ? C::kP(1) : C::kP(0));
+        const uint32_t o_addr = tmem_base + lane_base + (t ? C::kO(1) : C::kO(0));
         // (a scale of zero: the least normal number, which keeps what is masked at -infinity)
         const float scale_log2 = p.scale == 0.f ? 1.17549435e-38f : fabsf(p.scale) * kLog2e;
         int g = 0;                                   // running count of score tiles of this query tile
@@ -417,50 +449,55 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __gri
             const int idx = item_of_round(round, n_items);
             if (idx < 0) continue;
             const Item w = item_of(idx);
-            const int n = t ? w.blocks[1] : w.blocks[0];
-            if (t * shape.tokens >= w.tokens) continue;                     // no tokens in this tile
+            const int tile_end = t ? w.end[1] : w.end[0];                   // keys that some row of the tile sees
+            if (tile_end < 0) continue;                                     // no tokens in this tile
+            const int n = blocks_of(tile_end, C::kN);
             const int limit = p.causal ? min(w.keys - 1, w.last + token) : w.keys - 1;      // last visible key of this row
-            const int tile_end = p.causal ? min(w.keys, w.last + min(w.tokens, (t + 1) * shape.tokens)) : w.keys;
             const int all_see = p.causal ? min(w.keys, w.last + t * shape.tokens + 1) : w.keys;      // keys that every row of the tile sees
 
-            float m_ref = -INFINITY, l_sum = 0.f;
+            float m_ref = -INFINITY;
+            float2 rs[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};      // partial sums of the weights
             for (int j = 0; j < n; ++j, ++g) {
                 ok = mbar_wait_warp(&bar->s_full[t], g & 1, abort_flag, 0x800 + t);
                 if (!ok) break;
                 tc_fence_after();
-                const int k0 = j * kBlockN;
-                const int rest = tile_end - k0;                             // columns that some row sees
-                uint32_t s[4][32];
+                const int k0 = j * C::kN, rest = tile_end - k0;             // first key, and columns that some row sees
+                uint32_t s[C::kN];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + c * 32, s[c]);
+                for (int c = 0; c < C::kN / 32; ++c) tmem_ld32(s_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
+                if constexpr (C::kN % 32 != 0) tmem_ld16(s_addr + C::kN / 32 * 32, *reinterpret_cast<uint32_t(*)[16]>(&s[C::kN / 32 * 32]));
                 tmem_ld_wait();
-                if (k0 + kBlockN > all_see) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar->s_free[t]);                // the next block's scores may come
+                const bool masked = k0 + C::kN > all_see;
+                if (masked) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (k0 + c * 32 + i > limit) s[c][i] = 0xFF800000u;   // -inf
+                    for (int i = 0; i < C::kN; ++i)
+                        if (k0 + i > limit) s[i] = 0xFF800000u;             // -inf
                 }
                 // row max: 8 independent chains of 3-input max (one thread owns the whole row)
                 float mx8[8];
 #pragma unroll
                 for (int a = 0; a < 8; ++a) mx8[a] = -INFINITY;
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2)
-                        mx8[(i >> 1) & 7] = fmax3(mx8[(i >> 1) & 7], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
+                for (int i = 0; i < C::kN; i += 2) mx8[(i >> 1) & 7] = fmax3(mx8[(i >> 1) & 7], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
                 const float mx = fmaxf(fmax3(mx8[0], mx8[1], mx8[2]), fmaxf(fmax3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
                 const float m_cand = mx * scale_log2;
                 const bool grow = m_cand > m_ref + kRescale;
+                // The weights before these have been multiplied, and O is whole.  Looked at here, where the answer has time: it is yes nearly always.
+                bool taken = j == 0 || mbar_test(&bar->o_done[t], (g - 1) & 1);
+                auto wait_taken = [&]() {
+                    if (!__all_sync(0xFFFFFFFFu, taken)) ok = mbar_wait_warp(&bar->o_done[t], (g - 1) & 1, abort_flag, 0x900 + t);
+                    taken = true;
+                    tc_fence_after();
+                };
                 if (__any_sync(0xFFFFFFFFu, grow)) {
                     const float m_new = grow ? m_cand : m_ref;
                     const float alpha = (m_ref == -INFINITY) ? 0.f : fast_exp2(m_ref - m_new);
                     if (j > 0) {
-                        // all PV products issued so far for this tile must have landed in O
-                        ok = mbar_wait_warp(&bar->o_done[t], (g - 1) & 1, abort_flag, 0x900 + t);
+                        wait_taken();
                         if (!ok) break;
-                        tc_fence_after();
 #pragma unroll
                         for (int c = 0; c < D / 32; ++c) {
                             uint32_t o[32];
@@ -472,29 +509,39 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __gri
                         }
                         tmem_st_wait();
                     }
-                    l_sum *= alpha;
+#pragma unroll
+                    for (int a = 0; a < 4; ++a) { rs[a].x *= alpha; rs[a].y *= alpha; }
                     m_ref = m_new;
                 }
                 const float zero = m_ref == -INFINITY ? 0.f : m_ref - kLift;       // no key seen yet: weights of zero
-                float2 rs[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
                 const float2 sc2 = make_float2(scale_log2, scale_log2), nm2 = make_float2(-zero, -zero);
+                wait_taken();
+                if (!ok) break;
+                auto weigh = [&](int c, auto on_fma) {                      // columns [16 c, 16 c + 16); of each 8 pairs, the last `on_fma` off the special function unit
+                    uint32_t pk[8];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    if (c * 32 >= rest) break;
-                    uint32_t pk[16];
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        const float2 e = __ffma2_rn(make_float2(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1])), sc2, nm2);
-                        const float2 pp = make_float2(fast_exp2(e.x), fast_exp2(e.y));
+                    for (int i = 0; i < 16; i += 2) {
+                        const float2 e = __ffma2_rn(make_float2(__uint_as_float(s[16 * c + i]), __uint_as_float(s[16 * c + i + 1])), sc2, nm2);
+                        const float2 pp = i / 2 >= 8 - decltype(on_fma)::value ? exp2_fma(e) : make_float2(fast_exp2(e.x), fast_exp2(e.y));
                         rs[(i >> 1) & 3] = __fadd2_rn(rs[(i >> 1) & 3], pp);
                         pk[i >> 1] = Elem<T>::pack2(pp.x, pp.y);
                     }
-                    tmem_st16(s_addr + c * 16, pk);
+                    tmem_st8(p_addr + c * 8, pk);
+                };
+                if (!masked) {
+#pragma unroll
+                    for (int c = 0; c < C::kN / 16; ++c) weigh(c, std::integral_constant<int, C::kOnFma>());
+                } else {
+#pragma unroll
+                    for (int c = 0; c < C::kN / 16; ++c) {
+                        if (c * 16 >= rest) break;
+                        weigh(c, std::integral_constant<int, 0>());
+                    }
                 }
-                l_sum += ((rs[0].x + rs[0].y) + (rs[1].x + rs[1].y)) + ((rs[2].x + rs[2].y) + (rs[3].x + rs[3].y));
                 tmem_st_wait();
                 tc_fence_before();
-                mbar_arrive(&bar->p_ready[t]);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar->p_ready[t]);               // (one arrival per warp: those of 32 lanes take turns)
             }
             if (!ok) break;
 
@@ -504,6 +551,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __gri
                 if (!ok) break;
                 tc_fence_after();
             }
+            const float l_sum = ((rs[0].x + rs[0].y) + (rs[1].x + rs[1].y)) + ((rs[2].x + rs[2].y) + (rs[3].x + rs[3].y));
             const bool row_live = token < w.tokens;
             const float inv_l = l_sum == 0.f ? 0.f : 1.0f / l_sum;          // (a row that sees no key)
             const int hq = head_of(idx) + head_in;
@@ -614,8 +662,8 @@ int launch_t(cudaStream_t s, const PackedParams& p) {
     // no keys at all: no block is loaded, any map will do
     const View4 k = p.total_k > 0 ? p.k : p.q, v = p.total_k > 0 ? p.v : p.q;
     const int n_k = p.total_k > 0 ? p.total_k : p.total_q, h_k = p.total_k > 0 ? p.Hkv : p.Hq;
-    if (int rc = make_map(&maps.k, p.dtype, k, n_k, h_k, D, 1, kBlockN)) return rc;
-    if (int rc = make_map(&maps.v, p.dtype, v, n_k, h_k, D, 1, kBlockN)) return rc;
+    if (int rc = make_map(&maps.k, p.dtype, k, n_k, h_k, D, 1, Cfg<D>::kN)) return rc;
+    if (int rc = make_map(&maps.v, p.dtype, v, n_k, h_k, D, 1, Cfg<D>::kN)) return rc;
     packed_plan_kernel<<<1, kPlanThreads, 0, s>>>(p, shape.tokens, shape.max_items, plan, items, reinterpret_cast<int*>(ws + c.first));
     note_launch();
     VB200_CUDA_TRY(cudaPeekAtLastError());
