@@ -75,6 +75,8 @@ def test_norm_refuses_views(serving):
     assert call(q=view(capi, 8, 5, 128, P + 2)) == -3 and call(v_out=view(capi, 2, 5, 128, P + 8)) == -3
     assert call(k=capi.Tensor4(P, 2 * 5 * 128, 5 * 128 + 4, 128)) == -3
     assert call(rope=capi.Rope(1, None)) == -1
+    assert call(rope=capi.Rope(1, (C.c_float * 64)(*[1.0] * 63, float("inf")))) == -1
+    assert call(q=capi.Tensor4(P, 8 * 5 * 128, -5 * 128, 128)) == -3
     assert call(dst=serving.Rows(None, P, 0, 0)) == -1 and call(dst=serving.Rows(P, None, 0, 8)) == -1 and call(dst=serving.Rows(P, None, 2, 0)) == -1
 
 
@@ -203,8 +205,16 @@ def test_wrapper_refuses(serving):
         u = lambda n: torch.zeros(1, 1, 8, n, dtype=torch.uint8)  # noqa: E731
         serving.Kv4Cache(k_codes=u(64), v_codes=u(64), k_scales=u(4), v_scales=u(8))
     with pytest.raises(ValueError):
-        serving._like("k", x(2, 3), x(2, 4), (2, 4))
+        serving._view("k", x(1, 1, 2, 8), x(1, 1, 2, 8), (1, 1, 3, 8))
     with pytest.raises(ValueError):
-        serving._whole("rows", torch.zeros(4, 2, dtype=torch.int32).t(), torch.int32, torch.device("cpu"), 8)
+        serving._view("k", x(1, 1, 2, 8).float(), x(1, 1, 2, 8), (1, 1, 2, 8))
+    with pytest.raises(ValueError):
+        serving._view("k", x(1, 1, 8, 2).transpose(2, 3), x(1, 1, 2, 8), (1, 1, 2, 8))
+    with pytest.raises(ValueError):
+        serving._view3("k", x(2, 1, 8), x(2, 1, 8), (2, 2, 8))
+    with pytest.raises(ValueError):
+        serving._whole("rows", torch.zeros(4, 2, dtype=torch.int32).t(), torch.int32, -1, 8)
+    with pytest.raises(ValueError):
+        serving._whole("rows", torch.zeros(8, dtype=torch.int64), torch.int32, -1, 8)
     c = serving.Kv4Cache(2, 3, 60, 128, device="cpu")
     assert c.cap == 64 and c.view.stride_h == 64 and c.view.stride_b == 192

@@ -1,7 +1,6 @@
 // extern "C" entry points of vesper_b200_serving.h: argument validation, plans and workspaces.
 #include <algorithm>
 #include <cmath>
-#include <cstring>
 
 #include "hybrid.cuh"
 #include "serving.h"
@@ -13,9 +12,9 @@ namespace {
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
-// base and strides of a view on 16-byte boundaries; `batch`: stride_b counts too
+// base and strides of a view on 16-byte boundaries, none negative; `batch`: stride_b counts too
 bool view_aligned(const vb200_tensor4& t, int size, bool batch = true) {
-    auto ok = [&](int64_t s) { return (s * size) % 16 == 0; };
+    auto ok = [&](int64_t s) { return s >= 0 && (s * size) % 16 == 0; };
     return aligned16(t.ptr) && ok(t.stride_h) && ok(t.stride_s) && (!batch || ok(t.stride_b));
 }
 // the strides of dimensions of extent 1 are never used: any value may stand there
@@ -165,6 +164,9 @@ int vb200_qk_norm_rope(const vb200_qk_norm_rope_args* a) {
     if (a->start_pos < 0 || static_cast<int64_t>(a->start_pos) + a->T > INT32_MAX) return set_detail(VB200_ERR_INVALID_ARG, "start_pos out of range");
     if (a->norm && !(a->eps >= 0.f)) return set_detail(VB200_ERR_INVALID_ARG, "eps must be >= 0");
     if (a->rope.enabled && !a->rope.inv_freq_host) return set_detail(VB200_ERR_INVALID_ARG, "rope enabled without inv_freq_host");
+    if (a->rope.enabled)
+        for (int i = 0; i < a->D / 2; ++i)
+            if (!std::isfinite(a->rope.inv_freq_host[i])) return set_detail(VB200_ERR_INVALID_ARG, "inv_freq must be finite");
     if (int rc = check_rows(a->dst)) return rc;
     const int size = a->dtype == VB200_F32 ? 4 : 2;
     const bool scatter = a->dst.rows != nullptr;
@@ -189,7 +191,11 @@ int vb200_qk_norm_rope(const vb200_qk_norm_rope_args* a) {
     p.q_weight = a->norm ? a->q_weight : nullptr;
     p.k_weight = a->norm ? a->k_weight : nullptr;
     p.rope = a->rope.enabled; p.start_pos = a->start_pos; p.positions = a->positions;
-    if (p.rope) std::memcpy(p.inv_freq.v, a->rope.inv_freq_host, sizeof(float) * (a->D / 2));
+    if (p.rope)
+        for (int i = 0; i < a->D / 2; ++i) {
+            const long double turns = static_cast<long double>(a->rope.inv_freq_host[i]) / 6.283185307179586476925286766559L;
+            p.turns[i] = static_cast<unsigned long long>((turns - std::floor(turns)) * 18446744073709551616.0L);
+        }
     p.dst = row_map(a->dst);
     if (int rc = status_or_fail(p.status)) return rc;
     return launch_qk_norm_rope(static_cast<cudaStream_t>(a->stream), p);

@@ -6,7 +6,7 @@
 //
 // What bounds it: HBM, each element is read once and written once.  A row of D elements is held by D / 8 neighbouring threads, 8 elements each (16 bytes
 // of the 16-bit types), which sum the squares with shuffles.  A CTA takes a few tokens and a share of their heads: the angles of a token are computed once
-// per CTA and read from shared memory by all of its heads, and the rows of a packed projection lie next to each other.
+// per CTA, while its first rows are on their way, and read from shared memory by all of its heads; the rows of a packed projection lie next to each other.
 #include "serving.h"
 
 namespace vb200 {
@@ -14,7 +14,7 @@ namespace vb200 {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxTokens = 8;              // per CTA
+constexpr int kMaxTokens = 16;             // per CTA
 
 template <typename T> struct Row8 {        // 8 elements of a row
     uint4 raw;
@@ -40,94 +40,147 @@ template <> struct Row8<float> {
     __device__ void set(const float (&f)[8]) { a = make_float4(f[0], f[1], f[2], f[3]); b = make_float4(f[4], f[5], f[6], f[7]); }
 };
 
-// (cos, sin) of position * f: the product in 64 bits, brought into [-pi, pi] there, so that the fp32 functions see a small argument at any position
-__device__ __forceinline__ float2 turn_of(int position, float f) {
-    const double a = static_cast<double>(position) * static_cast<double>(f);
-    const double r = fma(-rint(a * 0.15915494309189535), 6.283185307179586, a);
+// (cos, sin) of position * inv_freq, given inv_freq as a fraction of a turn in 64 bits: the product's whole turns fall off the top, so that what is left is
+// good to 2^-33 of a turn at any position.  (In double precision, brought into [-pi, pi], the angles took as long as everything else: 8191 tokens of
+// 32 + 8 heads of 128 41 us, with 4 tokens per CTA 57.)
+__device__ __forceinline__ float2 turn_of(int position, unsigned long long fraction) {
+    const long long t = static_cast<long long>(static_cast<unsigned long long>(static_cast<long long>(position)) * fraction);
     float sn, cs;
-    sincosf(static_cast<float>(r), &sn, &cs);
+    sincospif(__int2float_rn(static_cast<int>(t >> 32)) * 4.656612873077393e-10f, &sn, &cs);      // 2^-31: half turns
     return make_float2(cs, sn);
 }
 
-// LANES: threads per row, the power of two at or above D / 8.  blockIdx.x: tokens, blockIdx.y: a share of the heads.
-template <typename T, int LANES>
-__global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(QkNormRopeParams p, int tokens_per_cta, int heads_per_cta, int heads) {
+// What a CTA has of its tokens: where their rows stand in the inputs and outputs (elements, without the head), and their angles.
+struct Tokens {
+    long long in[3][kMaxTokens], out[3][kMaxTokens];     // q, k, v; out -1: the token is left out
+    float4 turn[kMaxTokens][kMaxHalfDim / 2];            // (cos, sin) of two pairs
+};
+
+constexpr int kAhead = 2;                                // rows that a thread works on, while as many are on their way
+
+// The rows of one kind (0: q, 1: k, 2: v): heads [h0, h0 + n_heads) of n_tok tokens.  LANES: threads per row, the power of two at or above D / 8.
+template <typename T, int LANES, int KIND, typename F>
+__device__ __forceinline__ void rows_of(const QkNormRopeParams& p, const Tokens& tk, int n_tok, int h0, int n_heads, F before_first) {
     constexpr int kRows = kThreads / LANES;
-    __shared__ float2 turn[kMaxTokens][kMaxHalfDim];
-    __shared__ Place place[kMaxTokens];
+    const View4& in = KIND == 0 ? p.q : KIND == 1 ? p.k : p.v;
+    const View4& out = KIND == 0 ? p.q_out : KIND == 1 ? p.k_out : p.v_out;
+    const int lane = threadIdx.x % LANES, slot = threadIdx.x / LANES;
+    const bool live = lane * 8 < p.D;
+    const T* src = static_cast<const T*>(in.ptr) + h0 * in.sh + lane * 8;
+    T* dst = static_cast<T*>(out.ptr) + h0 * out.sh + lane * 8;
+    float w[8];
+    if (KIND < 2) {
+        const float* from = KIND == 0 ? p.q_weight : p.k_weight;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = 1.f;
+        if (from && live) {
+            const float4 x = reinterpret_cast<const float4*>(from)[2 * lane], y = reinterpret_cast<const float4*>(from)[2 * lane + 1];
+            w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w; w[4] = y.x; w[5] = y.y; w[6] = y.z; w[7] = y.w;
+        }
+    }
+    const int rows = n_tok * n_heads;
+    int r = slot / n_heads, h = slot - r * n_heads;      // token and head of the next row; then kRows on
+    const int step_r = kRows / n_heads, step_h = kRows - step_r * n_heads;
+    const float mean = 1.0f / p.D;
+    Row8<T> x[kAhead], nx[kAhead];
+    int at_r[kAhead], at_h[kAhead], nr[kAhead], nh[kAhead];
+    auto fetch = [&](int j0, Row8<T> (&y)[kAhead], int (&yr)[kAhead], int (&yh)[kAhead]) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            yr[u] = r; yh[u] = h;
+            if (j0 + u * kRows < rows && live) y[u].load(src + tk.in[KIND][r] + h * in.sh);
+            r += step_r; h += step_h;
+            if (h >= n_heads) { h -= n_heads; ++r; }
+        }
+    };
+    fetch(slot, x, at_r, at_h);
+    before_first();
+    for (int j0 = slot; j0 < rows; j0 += kAhead * kRows) {
+        fetch(j0 + kAhead * kRows, nx, nr, nh);          // the next rows are on their way while these are worked on
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            if (j0 + u * kRows >= rows) break;
+            if (KIND < 2) {
+                float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                if (live) x[u].get(f);
+                if (p.norm) {
+                    float sum = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) sum = fmaf(f[e], f[e], sum);
+                    // the threads of this row only: another row of the warp may be past the end
+                    const unsigned mask = ((1u << LANES) - 1u) << ((threadIdx.x & 31) / LANES * LANES);
+#pragma unroll
+                    for (int o = LANES / 2; o >= 1; o >>= 1) sum += __shfl_xor_sync(mask, sum, o);
+                    const float inv = rsqrtf(fmaf(sum, mean, p.eps));
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) f[e] *= inv * w[e];
+                }
+                if (p.rope && live) {
+                    const float4 c0 = tk.turn[at_r[u]][2 * lane], c1 = tk.turn[at_r[u]][2 * lane + 1];
+                    const float cosine[4] = {c0.x, c0.z, c1.x, c1.z}, sine[4] = {c0.y, c0.w, c1.y, c1.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float a = f[2 * e], c = f[2 * e + 1];
+                        f[2 * e] = a * cosine[e] - c * sine[e];
+                        f[2 * e + 1] = a * sine[e] + c * cosine[e];
+                    }
+                }
+                x[u].set(f);
+            }
+            const long long to = tk.out[KIND][at_r[u]];
+            if (live && to >= 0) x[u].store(dst + to + at_h[u] * out.sh);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) { x[u] = nx[u]; at_r[u] = nr[u]; at_h[u] = nh[u]; }
+    }
+}
+
+// blockIdx.x: tokens, blockIdx.y: a share of the heads of q, k and v together
+template <typename T, int LANES>
+__global__ void __launch_bounds__(kThreads, 4) qk_norm_rope_kernel(QkNormRopeParams p, int tokens_per_cta, int heads_per_cta, int heads) {
+    __shared__ Tokens tk;
     const int half = p.D / 2;
     const int total = p.B * p.T;
     const int i0 = blockIdx.x * tokens_per_cta, n_tok = min(tokens_per_cta, total - i0);
-    const int h0 = blockIdx.y * heads_per_cta, n_heads = min(heads_per_cta, heads - h0);
-    const int lane = threadIdx.x % LANES, slot = threadIdx.x / LANES;
-    const bool live = lane * 8 < p.D;
-
-    if (p.rope)
-        for (int j = threadIdx.x; j < n_tok * half; j += kThreads) {
-            const int r = j / half, e = j - r * half;
-            const int pos = p.positions ? p.positions[i0 + r] : p.start_pos + (i0 + r) % p.T;
-            turn[r][e] = turn_of(pos, p.inv_freq.v[e]);
-        }
-    if (p.dst.rows && threadIdx.x < n_tok) place[threadIdx.x] = find_place(p.dst, (i0 + threadIdx.x) / p.T, (i0 + threadIdx.x) % p.T, p.T, p.status);
-    __syncthreads();
-
-    for (int j = slot; j < n_tok * n_heads; j += kRows) {
-        const int r = j / n_heads;
-        int h = h0 + j - r * n_heads;
-        const int b = (i0 + r) / p.T, t = (i0 + r) % p.T;
-        const int n_q = p.q.ptr ? p.Hq : 0, n_k = p.k.ptr ? p.Hkv : 0;
-        const int kind = h < n_q ? 0 : h < n_q + n_k ? 1 : 2;              // q, k, v
-        h -= kind == 0 ? 0 : kind == 1 ? n_q : n_q + n_k;
-        const View4& in = kind == 0 ? p.q : kind == 1 ? p.k : p.v;
-        const View4& out = kind == 0 ? p.q_out : kind == 1 ? p.k_out : p.v_out;
-        long long to = b * out.sb + h * out.sh + t * out.ss;
-        bool keep = live;
-        if (kind != 0 && p.dst.rows) {
-            to = place[r].seq * out.sb + h * out.sh + place[r].row * out.ss;
-            keep = live && place[r].row >= 0;
-        }
-        Row8<T> x;
-        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (live) {
-            x.load(static_cast<const T*>(in.ptr) + b * in.sb + h * in.sh + t * in.ss + lane * 8);
-            x.get(f);
-        }
-        if (kind != 2) {
-            if (p.norm) {
-                float sum = 0.f;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) sum = fmaf(f[e], f[e], sum);
-                // the rows of a warp that is past the end are not here: name the threads of this row only
-                const unsigned mask = LANES == 32 ? 0xFFFFFFFFu : ((1u << LANES) - 1u) << ((threadIdx.x & 31) / LANES * LANES);
-#pragma unroll
-                for (int o = LANES / 2; o >= 1; o >>= 1) sum += __shfl_xor_sync(mask, sum, o);
-                const float inv = rsqrtf(sum / p.D + p.eps);
-                const float* w = kind == 0 ? p.q_weight : p.k_weight;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] *= inv;
-                if (w && live)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) f[e] *= w[lane * 8 + e];
-            }
-            if (p.rope && live)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float2 cs = turn[r][lane * 4 + e];
-                    const float a = f[2 * e], c = f[2 * e + 1];
-                    f[2 * e] = a * cs.x - c * cs.y;
-                    f[2 * e + 1] = a * cs.y + c * cs.x;
-                }
-            x.set(f);
-        }
-        if (keep) x.store(static_cast<T*>(out.ptr) + to + lane * 8);
+    const int h0 = blockIdx.y * heads_per_cta, h1 = min(h0 + heads_per_cta, heads);
+    if (threadIdx.x < n_tok) {
+        const int i = i0 + threadIdx.x, b = i / p.T, t = i - b * p.T;
+        tk.in[0][threadIdx.x] = b * p.q.sb + t * p.q.ss;
+        tk.in[1][threadIdx.x] = b * p.k.sb + t * p.k.ss;
+        tk.in[2][threadIdx.x] = b * p.v.sb + t * p.v.ss;
+        tk.out[0][threadIdx.x] = b * p.q_out.sb + t * p.q_out.ss;
+        Place c{b, t};
+        if (p.dst.rows) c = find_place(p.dst, b, t, p.T, p.status);
+        tk.out[1][threadIdx.x] = c.row < 0 ? -1 : c.seq * p.k_out.sb + c.row * p.k_out.ss;
+        tk.out[2][threadIdx.x] = c.row < 0 ? -1 : c.seq * p.v_out.sb + c.row * p.v_out.ss;
     }
+    __syncthreads();
+    bool angles = !p.rope;
+    auto find_angles = [&]() {                           // while the first rows are on their way; the whole block comes here
+        if (angles) return;
+        angles = true;
+        for (int i = threadIdx.x; i < n_tok * half; i += kThreads) {
+            const int r = i / half, e = i - r * half;
+            const int pos = p.positions ? p.positions[i0 + r] : p.start_pos + (i0 + r) % p.T;
+            reinterpret_cast<float2*>(tk.turn[r])[e] = turn_of(pos, p.turns[e]);
+        }
+        __syncthreads();
+    };
+    const int n_q = p.q.ptr ? p.Hq : 0, n_k = p.k.ptr ? p.Hkv : 0;
+    if (h0 < n_q) rows_of<T, LANES, 0>(p, tk, n_tok, h0, min(h1, n_q) - h0, find_angles);
+    const int k0 = max(h0, n_q) - n_q, k1 = min(h1 - n_q, n_k);
+    if (k0 < k1) rows_of<T, LANES, 1>(p, tk, n_tok, k0, k1 - k0, find_angles);
+    const int v0 = max(h0, n_q + n_k) - n_q - n_k, v1 = h1 - n_q - n_k;
+    if (v0 < v1) rows_of<T, LANES, 2>(p, tk, n_tok, v0, v1 - v0, [] {});
 }
 
 template <typename T, int LANES>
 int launch_t(cudaStream_t s, const QkNormRopeParams& p) {
     const int heads = (p.q.ptr ? p.Hq : 0) + (p.k.ptr ? p.Hkv : 0) + (p.v.ptr ? p.Hkv : 0);
     const long long total = static_cast<long long>(p.B) * p.T;
-    int tokens = kMaxTokens;
+    // Tokens per CTA: 16 where that leaves four rounds of four CTAs per SM (65536 tokens of 32 + 8 heads of 128: 262 us, with 8 273), 8 else (8191 tokens:
+    // 39.7 us, with 16 44.5), fewer where there are not two CTAs per SM.
+    int tokens = (total + 15) / 16 >= 4 * 592 ? 16 : 8;
     while (tokens > 1 && (total + tokens - 1) / tokens < 296) tokens >>= 1;
     const long long blocks = (total + tokens - 1) / tokens;
     long long shares = (296 + blocks - 1) / blocks;

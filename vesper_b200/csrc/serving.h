@@ -42,7 +42,7 @@ struct QkNormRopeParams {
     int rope, start_pos;
     const int* positions;
     RowMap dst;
-    InvFreq inv_freq;
+    unsigned long long turns[kMaxHalfDim]; // inv_freq / (2 pi) as a fraction of 2^64, whole turns dropped
     int* status;
 };
 int launch_qk_norm_rope(cudaStream_t s, const QkNormRopeParams& p);

@@ -63,45 +63,69 @@ def load():
     return _lib
 
 
-def _stream(t, stream):
+_TYPES = {}
+_NONE4 = capi.Tensor4(None, 0, 0, 0)
+
+
+def _code(t):
+    """vb200_dtype of a tensor's type."""
+    if not _TYPES:
+        import torch
+        _TYPES.update({torch.float32: capi.F32, torch.bfloat16: capi.BF16, torch.float16: capi.F16})
+    return _TYPES[t.dtype]
+
+
+def _stream(device, stream):
+    """The raw handle of `stream`, or of the device's current one."""
+    if stream is not None:
+        return stream.cuda_stream
     import torch
-    return (stream if stream is not None else torch.cuda.current_stream(t.device)).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _like(name, t, model, shape):
-    """`t` has to be of the model's type and device and of this shape."""
-    if t is not None and (t.dtype != model.dtype or t.device != model.device or tuple(t.shape) != tuple(shape)):
-        raise ValueError(f"{name}: expected {tuple(shape)} {model.dtype} on {model.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
-    if t is not None and t.stride(-1) != 1:
-        raise ValueError(f"{name}: the last dimension must be contiguous")
+def _wrong(name, t, shape, model):
+    raise ValueError(f"{name}: expected {tuple(shape)} {model.dtype} on {model.device}, the last dimension contiguous, got {tuple(t.shape)} {t.dtype} on {t.device}, "
+                     f"strides {t.stride()}")
+
+
+def _view(name, t, model, shape):
+    """The view of a 4-D tensor, which has to be of the model's type and device and of this shape."""
+    s = t.stride()
+    if t.shape != shape or t.dtype is not model.dtype or t.get_device() != model.get_device() or s[3] != 1:
+        _wrong(name, t, shape, model)
+    return capi.Tensor4(t.data_ptr(), s[0], s[1], s[2])
+
+
+def _view3(name, t, model, shape):
+    """[tokens, H, D] -> the view the packed operators take."""
+    s = t.stride()
+    if t.shape != shape or t.dtype is not model.dtype or t.get_device() != model.get_device() or s[2] != 1:
+        _wrong(name, t, shape, model)
+    return capi.Tensor4(t.data_ptr(), 0, s[1], s[0])
 
 
 def _whole(name, t, dtype, device, numel):
-    """An array of the device that the kernels read as it lies."""
-    if t is not None and (t.dtype != dtype or t.device != device or t.numel() != numel or not t.is_contiguous()):
-        raise ValueError(f"{name}: expected {numel} contiguous {dtype} on {device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
-
-
-def _view3(t):
-    """[tokens, H, D] -> the view the packed operators take."""
-    return capi.Tensor4(t.data_ptr(), 0, t.stride(1), t.stride(0))
+    """The address of an array that the kernels read as it lies (None: none)."""
+    if t is None:
+        return None
+    if t.dtype is not dtype or t.get_device() != device or t.numel() != numel or not t.is_contiguous():
+        raise ValueError(f"{name}: expected {numel} contiguous {dtype} on device {device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    return t.data_ptr()
 
 
 def _rows(rows, seqs, device, tokens, n_seqs, cap):
     import torch
-    _whole("rows", rows, torch.int32, device, tokens)
-    _whole("seqs", seqs, torch.int32, device, tokens)
-    return Rows(_ptr(rows), _ptr(seqs), n_seqs, cap)
+    return Rows(_whole("rows", rows, torch.int32, device, tokens), _whole("seqs", seqs, torch.int32, device, tokens), n_seqs, cap)
 
 
 def _workspace(workspace, need, t, stream):
     if workspace is None:
         workspace = capi._workspace(need, t.device, stream)
-    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
 def qk_norm_rope(q, k, v=None, *, eps=None, q_weight=None, k_weight=None, theta=None, inv_freq=None, start_pos=0, positions=None, q_out=None, k_out=None, v_out=None,
@@ -114,33 +138,28 @@ def qk_norm_rope(q, k, v=None, *, eps=None, q_weight=None, k_weight=None, theta=
     if some is None:
         raise ValueError("qk_norm_rope: one of q, k, v must be given")
     B, _, T, D = some.shape
+    device, scatter = some.get_device(), rows is not None
     kv = k if k is not None else v
-    a = QkNormRopeArgs(struct_size=C.sizeof(QkNormRopeArgs), device=some.device.index, stream=_stream(some, stream), dtype=capi.dtype_code(some), B=B,
-                       Hq=q.shape[1] if q is not None else 0, Hkv=kv.shape[1] if kv is not None else 0, T=T, D=D, start_pos=start_pos)
-    scatter = rows is not None
-    if not scatter and v is not None and v_out is None:
-        raise ValueError("qk_norm_rope: v needs v_out")
+    Hq, Hkv = q.shape[1] if q is not None else 0, kv.shape[1] if kv is not None else 0
     q_out = q if q_out is None else q_out
     k_out = k if k_out is None and not scatter else k_out
-    for name, t, to, H in (("q", q, q_out, a.Hq), ("k", k, k_out, a.Hkv), ("v", v, v_out, a.Hkv)):
-        _like(name, t, some, (B, H, T, D))
-        cached = scatter and name != "q" and to is not None
-        _like(name + "_out", to, some, (to.shape[0], H, to.shape[2], D) if cached else (B, H, T, D))
-        setattr(a, name, capi.view4(t))
-        setattr(a, name + "_out", capi.view4(to))
+    if not scatter and v is not None and v_out is None:
+        raise ValueError("qk_norm_rope: v needs v_out")
+    dst, kv_out_shape = Rows(), (B, Hkv, T, D)
     if scatter:
         cache = k_out if k_out is not None else v_out
         if cache is None:
             raise ValueError("qk_norm_rope: rows need k_out or v_out")
-        if k_out is not None and v_out is not None and (k_out.shape[0], k_out.shape[2]) != (v_out.shape[0], v_out.shape[2]):
-            raise ValueError("qk_norm_rope: k_out and v_out must have the same sequences and rows")
-        a.dst = _rows(rows, seqs, some.device, B * T, cache.shape[0], cache.shape[2])
-    _whole("positions", positions, torch.int32, some.device, B * T)
-    a.positions = _ptr(positions)
+        kv_out_shape = (cache.shape[0], Hkv, cache.shape[2], D)
+        dst = _rows(rows, seqs, device, B * T, cache.shape[0], cache.shape[2])
+    elif seqs is not None:
+        raise ValueError("qk_norm_rope: seqs need rows")
+    views = [_NONE4 if t is None else _view(name, t, some, shape) for name, t, shape in (
+        ("q", q, (B, Hq, T, D)), ("k", k, (B, Hkv, T, D)), ("v", v, (B, Hkv, T, D)), ("q_out", q_out, (B, Hq, T, D)), ("k_out", k_out, kv_out_shape), ("v_out", v_out, kv_out_shape))]
+    qw = kw = None
     if eps is not None:
-        _whole("q_weight", q_weight, torch.float32, some.device, D)
-        _whole("k_weight", k_weight, torch.float32, some.device, D)
-        a.norm, a.eps, a.q_weight, a.k_weight = 1, eps, _ptr(q_weight), _ptr(k_weight)
+        qw, kw = _whole("q_weight", q_weight, torch.float32, device, D), _whole("k_weight", k_weight, torch.float32, device, D)
+    rope = capi.Rope(0, None)
     if inv_freq is None and theta is not None:
         inv_freq = capi.inv_freq(theta, D)
     if inv_freq is not None:
@@ -149,13 +168,17 @@ def qk_norm_rope(q, k, v=None, *, eps=None, q_weight=None, k_weight=None, theta=
         if not isinstance(inv_freq, C.Array):
             import numpy as np
             inv_freq = (C.c_float * (D // 2)).from_buffer_copy(np.ascontiguousarray(inv_freq, dtype=np.float32))
-        a.rope = capi.Rope(1, inv_freq)
-    capi.check(load().vb200_qk_norm_rope(C.byref(a)))
+        rope = capi.Rope(1, inv_freq)
+    a = QkNormRopeArgs(C.sizeof(QkNormRopeArgs), device, _stream(device, stream), _code(some), B, Hq, Hkv, T, D, *views, int(eps is not None), eps or 0.0, qw, kw, rope, start_pos,
+                       _whole("positions", positions, torch.int32, device, B * T), dst)
+    rc = load().vb200_qk_norm_rope(C.byref(a))
+    if rc:
+        capi.check(rc)
     return q_out, k_out, v_out
 
 
 def _packed_args(q, k, batch):
-    return PackedArgs(struct_size=C.sizeof(PackedArgs), device=q.device.index, dtype=capi.dtype_code(q), batch=batch, Hq=q.shape[1], Hkv=k.shape[1], D=q.shape[2],
+    return PackedArgs(struct_size=C.sizeof(PackedArgs), device=q.get_device(), dtype=_code(q), batch=batch, Hq=q.shape[1], Hkv=k.shape[1], D=q.shape[2],
                       total_q=q.shape[0], total_k=k.shape[0])
 
 
@@ -167,25 +190,19 @@ def prefill_packed_workspace(q, k, *, batch):
 def prefill_packed(q, k, v, o=None, lse=None, *, scale, cu_seqlens_q, cu_seqlens_k=None, causal=True, workspace=None, stream=None):
     """vb200_prefill_packed_fwd: q [total_q, Hq, D], k, v [total_k, Hkv, D], cu_seqlens int32 [batch + 1] on the device, lse [Hq, total_q] fp32.  Returns o."""
     import torch
-    o = torch.empty_like(q) if o is None else o
-    batch = cu_seqlens_q.numel() - 1
-    _like("q", q, q, q.shape)
-    _like("k", k, q, (k.shape[0], k.shape[1], q.shape[2]))
-    _like("v", v, q, k.shape)
-    _like("o", o, q, q.shape)
-    _whole("lse", lse, torch.float32, q.device, q.shape[0] * q.shape[1])
-    _whole("cu_seqlens_q", cu_seqlens_q, torch.int32, q.device, batch + 1)
-    _whole("cu_seqlens_k", cu_seqlens_k, torch.int32, q.device, batch + 1)
-    if cu_seqlens_k is None and k.shape[0] < q.shape[0]:
+    o = torch.empty_like(q, memory_format=torch.contiguous_format) if o is None else o
+    (tq, Hq, D), (tk, Hkv, _) = q.shape, k.shape
+    device, batch = q.get_device(), cu_seqlens_q.numel() - 1
+    if cu_seqlens_k is None and tk < tq:
         raise ValueError("prefill_packed: fewer keys than queries need cu_seqlens_k")
-    a = _packed_args(q, k, batch)
-    a.stream, a.causal, a.scale = _stream(q, stream), int(causal), scale
-    a.q, a.o, a.k, a.v, a.lse = _view3(q), _view3(o), _view3(k), _view3(v), _ptr(lse)
-    a.cu_seqlens_q, a.cu_seqlens_k = _ptr(cu_seqlens_q), _ptr(cu_seqlens_k)
+    a = PackedArgs(C.sizeof(PackedArgs), device, _stream(device, stream), _code(q), batch, Hq, Hkv, D, tq, tk, int(causal), scale, _view3("q", q, q, (tq, Hq, D)),
+                   _view3("o", o, q, (tq, Hq, D)), _view3("k", k, q, (tk, Hkv, D)), _view3("v", v, q, (tk, Hkv, D)), _whole("lse", lse, torch.float32, device, tq * Hq),
+                   _whole("cu_seqlens_q", cu_seqlens_q, torch.int32, device, batch + 1), _whole("cu_seqlens_k", cu_seqlens_k, torch.int32, device, batch + 1))
     L = load()
-    need = L.vb200_prefill_packed_workspace_bytes(C.byref(a)) if workspace is None else 0
-    workspace, a.workspace, a.workspace_bytes = _workspace(workspace, need, q, stream)
-    capi.check(L.vb200_prefill_packed_fwd(C.byref(a)))
+    a.workspace, a.workspace_bytes = _workspace(workspace, 0 if workspace is not None else L.vb200_prefill_packed_workspace_bytes(C.byref(a)), q, stream)
+    rc = L.vb200_prefill_packed_fwd(C.byref(a))
+    if rc:
+        capi.check(rc)
     return o
 
 
@@ -207,6 +224,7 @@ class Kv4Cache:
                 raise ValueError(f"Kv4Cache: {name} must be uint8 [{self.seqs}, {self.Hkv}, {self.cap}, {n}] with contiguous rows")
             if any(t.shape[d] > 1 and t.stride(d) * row != k_codes.stride(d) * n for d in (0, 1)):
                 raise ValueError("Kv4Cache: codes and scales must have the same strides, in rows")
+        self.device = k_codes.get_device()
         self.view = Kv4CacheView(_ptr(k_codes), _ptr(v_codes), _ptr(k_scales), _ptr(v_scales), k_codes.stride(0) // row, k_codes.stride(1) // row, self.seqs, self.cap,
                                  k_exponent, v_exponent)
 
@@ -215,13 +233,16 @@ class Kv4Cache:
         if some is None:
             raise ValueError("Kv4Cache: k and v are both missing")
         B, _, T, _ = some.shape
-        for name, t in (("k", k), ("v", v)):
-            _like(name, t, some, (B, self.Hkv, T, self.D))
-        if some.device != self.k_codes.device:
+        shape, device = (B, self.Hkv, T, self.D), some.get_device()
+        if device != self.device:
             raise ValueError(f"Kv4Cache: rows on {some.device}, cache on {self.k_codes.device}")
-        a = Kv4RowsArgs(struct_size=C.sizeof(Kv4RowsArgs), device=some.device.index, stream=_stream(some, stream), dtype=capi.dtype_code(some), B=B, Hkv=self.Hkv, T=T, D=self.D,
-                        k=capi.view4(k), v=capi.view4(v), cache=self.view, start_row=start_row, at=_rows(rows, seqs, some.device, B * T, self.seqs, self.cap))
-        capi.check(entry(C.byref(a)))
+        if seqs is not None and rows is None:
+            raise ValueError("Kv4Cache: seqs need rows")
+        a = Kv4RowsArgs(C.sizeof(Kv4RowsArgs), device, _stream(device, stream), _code(some), B, self.Hkv, T, self.D, _NONE4 if k is None else _view("k", k, some, shape),
+                        _NONE4 if v is None else _view("v", v, some, shape), self.view, start_row, _rows(rows, seqs, device, B * T, self.seqs, self.cap))
+        rc = entry(C.byref(a))
+        if rc:
+            capi.check(rc)
 
     def append(self, k, v, *, start_row=0, rows=None, seqs=None, stream=None):
         """vb200_kv4_append: [B, Hkv, T, D] keys and values into rows start_row + t of sequence b, or where rows (and seqs) [B, T] int32 say."""
@@ -233,7 +254,7 @@ class Kv4Cache:
 
 
 def _decode_args(q, cache, max_len, num_splits):
-    return DecodeKv4Args(struct_size=C.sizeof(DecodeKv4Args), device=q.device.index, dtype=capi.dtype_code(q), B=q.shape[0], Hq=q.shape[1], Hkv=cache.Hkv, D=q.shape[3],
+    return DecodeKv4Args(struct_size=C.sizeof(DecodeKv4Args), device=q.get_device(), dtype=_code(q), B=q.shape[0], Hq=q.shape[1], Hkv=cache.Hkv, D=q.shape[3],
                          cache=cache.view, max_len=max_len, num_splits=num_splits)
 
 
@@ -247,21 +268,17 @@ def decode_kv4_workspace(q, cache, *, max_len=0, num_splits=0, whole_generation=
 def decode_kv4(q, o, cache, *, scale, k_new=None, v_new=None, lse=None, seq_lens=None, uniform_len=0, advance_lens=False, max_len=0, num_splits=0, workspace=None, stream=None):
     """vb200_decode_kv4_fwd: one token per sequence, q and o [B, Hq, 1, D], k_new and v_new [B, Hkv, 1, D] appended first, seq_lens int32 [B] on the device."""
     import torch
-    B = q.shape[0]
-    _like("q", q, q, (B, q.shape[1], 1, cache.D))
-    _like("o", o, q, q.shape)
-    _like("k_new", k_new, q, (B, cache.Hkv, 1, cache.D))
-    _like("v_new", v_new, q, (B, cache.Hkv, 1, cache.D))
-    _whole("lse", lse, torch.float32, q.device, B * q.shape[1])
-    _whole("seq_lens", seq_lens, torch.int32, q.device, B)
-    if q.device != cache.k_codes.device:
+    B, Hq = q.shape[0], q.shape[1]
+    device, shape, new = q.get_device(), (B, Hq, 1, cache.D), (B, cache.Hkv, 1, cache.D)
+    if device != cache.device:
         raise ValueError(f"decode_kv4: q on {q.device}, cache on {cache.k_codes.device}")
-    a = _decode_args(q, cache, max_len, num_splits)
-    a.stream, a.scale = _stream(q, stream), scale
-    a.q, a.o, a.lse, a.k_new, a.v_new = capi.view4(q), capi.view4(o), _ptr(lse), capi.view4(k_new), capi.view4(v_new)
-    a.seq_lens, a.uniform_len, a.advance_lens = _ptr(seq_lens), uniform_len, int(advance_lens)
+    a = DecodeKv4Args(C.sizeof(DecodeKv4Args), device, _stream(device, stream), _code(q), B, Hq, cache.Hkv, cache.D, scale, _view("q", q, q, shape),
+                      _NONE4 if k_new is None else _view("k_new", k_new, q, new), _NONE4 if v_new is None else _view("v_new", v_new, q, new), _view("o", o, q, shape),
+                      _whole("lse", lse, torch.float32, device, B * Hq), cache.view, _whole("seq_lens", seq_lens, torch.int32, device, B), uniform_len, int(advance_lens),
+                      max_len, num_splits)
     L = load()
-    need = L.vb200_decode_kv4_workspace_bytes(C.byref(a)) if workspace is None else 0
-    workspace, a.workspace, a.workspace_bytes = _workspace(workspace, need, q, stream)
-    capi.check(L.vb200_decode_kv4_fwd(C.byref(a)))
+    a.workspace, a.workspace_bytes = _workspace(workspace, 0 if workspace is not None else L.vb200_decode_kv4_workspace_bytes(C.byref(a)), q, stream)
+    rc = L.vb200_decode_kv4_fwd(C.byref(a))
+    if rc:
+        capi.check(rc)
     return o
