@@ -4,10 +4,13 @@
 //   (z[2i], z[2i+1]) = rotation of (y[2i], y[2i+1]) by position * inv_freq[i]
 // q and k come out turned, v is copied; k and v go to plain tensors or to rows of a cache.
 //
-// What bounds it: HBM, each element is read once and written once.  A row of D elements is held by D / 8 neighbouring threads, 8 elements each (16 bytes
-// of the 16-bit types), which sum the squares with shuffles.  A CTA takes a few tokens and a share of their heads: the angles of a token are computed once
+// What bounds it: HBM, each element is read once and written once.  A row of D elements is held by D / 16 neighbouring threads, 16 elements each, which
+// sum the squares with shuffles.  A CTA takes a few tokens and a share of their heads: the angles of a token are computed once
 // per CTA, while its first rows are on their way, and read from shared memory by all of its heads; the rows of a packed projection lie next to each other.
+#include "hybrid.cuh"
 #include "serving.h"
+
+#include <algorithm>
 
 namespace vb200 {
 
@@ -56,88 +59,127 @@ struct Tokens {
     float4 turn[kMaxTokens][kMaxHalfDim / 2];            // (cos, sin) of two pairs
 };
 
-constexpr int kAhead = 2;                                // rows that a thread works on, while as many are on their way
+constexpr int kAhead = 1;                                // rows that a thread works on, while as many are on their way
 
-// The rows of one kind (0: q, 1: k, 2: v): heads [h0, h0 + n_heads) of n_tok tokens.  LANES: threads per row, the power of two at or above D / 8.
+// The rows of one kind (0: q, 1: k, 2: v): heads [h0, h0 + n_heads) of n_tok tokens.  LANES: threads per row, the power of two at or above D / 16; a thread has
+// the elements [8 lane, 8 lane + 8) and those 8 LANES further on.
 template <typename T, int LANES, int KIND, typename F>
 __device__ __forceinline__ void rows_of(const QkNormRopeParams& p, const Tokens& tk, int n_tok, int h0, int n_heads, F before_first) {
     constexpr int kRows = kThreads / LANES;
     const View4& in = KIND == 0 ? p.q : KIND == 1 ? p.k : p.v;
     const View4& out = KIND == 0 ? p.q_out : KIND == 1 ? p.k_out : p.v_out;
     const int lane = threadIdx.x % LANES, slot = threadIdx.x / LANES;
-    const bool live = lane * 8 < p.D;
+    const bool live[2] = {lane * 8 < p.D, (lane + LANES) * 8 < p.D};
     const T* src = static_cast<const T*>(in.ptr) + h0 * in.sh + lane * 8;
     T* dst = static_cast<T*>(out.ptr) + h0 * out.sh + lane * 8;
-    float w[8];
+    float w[2][8];
     if (KIND < 2) {
         const float* from = KIND == 0 ? p.q_weight : p.k_weight;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = 1.f;
-        if (from && live) {
-            const float4 x = reinterpret_cast<const float4*>(from)[2 * lane], y = reinterpret_cast<const float4*>(from)[2 * lane + 1];
-            w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w; w[4] = y.x; w[5] = y.y; w[6] = y.z; w[7] = y.w;
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[c][e] = 1.f;
+            if (from && live[c]) {
+                const float4* f4 = reinterpret_cast<const float4*>(from) + 2 * (lane + c * LANES);
+                const float4 x = f4[0], y = f4[1];
+                w[c][0] = x.x; w[c][1] = x.y; w[c][2] = x.z; w[c][3] = x.w; w[c][4] = y.x; w[c][5] = y.y; w[c][6] = y.z; w[c][7] = y.w;
+            }
         }
     }
     const int rows = n_tok * n_heads;
     int r = slot / n_heads, h = slot - r * n_heads;      // token and head of the next row; then kRows on
     const int step_r = kRows / n_heads, step_h = kRows - step_r * n_heads;
     const float mean = 1.0f / p.D;
-    Row8<T> x[kAhead], nx[kAhead];
-    int at_r[kAhead], at_h[kAhead], nr[kAhead], nh[kAhead];
-    auto fetch = [&](int j0, Row8<T> (&y)[kAhead], int (&yr)[kAhead], int (&yh)[kAhead]) {
+    struct Row {
+        Row8<T> c[2];
+        int r, h;
+    };
+    Row x[kAhead], next[kAhead];
+    auto fetch = [&](int j0, Row (&y)[kAhead]) {
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            yr[u] = r; yh[u] = h;
-            if (j0 + u * kRows < rows && live) y[u].load(src + tk.in[KIND][r] + h * in.sh);
+            y[u].r = r; y[u].h = h;
+            if (j0 + u * kRows < rows) {
+                const T* from = src + (tk.in[KIND][r] + h * in.sh);
+                if (live[0]) y[u].c[0].load(from);
+                if (live[1]) y[u].c[1].load(from + LANES * 8);
+            }
             r += step_r; h += step_h;
             if (h >= n_heads) { h -= n_heads; ++r; }
         }
     };
-    fetch(slot, x, at_r, at_h);
+    fetch(slot, x);
     before_first();
     for (int j0 = slot; j0 < rows; j0 += kAhead * kRows) {
-        fetch(j0 + kAhead * kRows, nx, nr, nh);          // the next rows are on their way while these are worked on
+        fetch(j0 + kAhead * kRows, next);                // the next rows are on their way while these are worked on
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
             if (j0 + u * kRows >= rows) break;
             if (KIND < 2) {
-                float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                if (live) x[u].get(f);
-                if (p.norm) {
-                    float sum = 0.f;
+                float f[2][8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) sum = fmaf(f[e], f[e], sum);
+                for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) f[c][e] = 0.f;
+                    if (live[c]) x[u].c[c].get(f[c]);
+                }
+                if (p.norm) {
+                    float2 sum2 = make_float2(0.f, 0.f);
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int e = 0; e < 8; e += 2) {
+                            const float2 y = make_float2(f[c][e], f[c][e + 1]);
+                            sum2 = __ffma2_rn(y, y, sum2);
+                        }
+                    float sum = sum2.x + sum2.y;
                     // the threads of this row only: another row of the warp may be past the end
                     const unsigned mask = ((1u << LANES) - 1u) << ((threadIdx.x & 31) / LANES * LANES);
 #pragma unroll
                     for (int o = LANES / 2; o >= 1; o >>= 1) sum += __shfl_xor_sync(mask, sum, o);
                     const float inv = rsqrtf(fmaf(sum, mean, p.eps));
+                    const float2 inv2 = make_float2(inv, inv);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) f[e] *= inv * w[e];
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int e = 0; e < 8; e += 2) {
+                            const float2 y = __fmul2_rn(make_float2(f[c][e], f[c][e + 1]), __fmul2_rn(inv2, make_float2(w[c][e], w[c][e + 1])));
+                            f[c][e] = y.x; f[c][e + 1] = y.y;
+                        }
                 }
-                if (p.rope && live) {
-                    const float4 c0 = tk.turn[at_r[u]][2 * lane], c1 = tk.turn[at_r[u]][2 * lane + 1];
-                    const float cosine[4] = {c0.x, c0.z, c1.x, c1.z}, sine[4] = {c0.y, c0.w, c1.y, c1.w};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float a = f[2 * e], c = f[2 * e + 1];
-                        f[2 * e] = a * cosine[e] - c * sine[e];
-                        f[2 * e + 1] = a * sine[e] + c * cosine[e];
+                for (int c = 0; c < 2; ++c) {
+                    if (!live[c]) continue;
+                    if (p.rope) {
+                        const float4* at = tk.turn[x[u].r] + 2 * (lane + c * LANES);
+                        const float4 c0 = at[0], c1 = at[1];
+                        const float2 cs[4] = {{c0.x, c0.y}, {c0.z, c0.w}, {c1.x, c1.y}, {c1.z, c1.w}};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            // (a cos - b sin, b cos + a sin)
+                            const float a = f[c][2 * e], b = f[c][2 * e + 1];
+                            const float2 y = __ffma2_rn(make_float2(a, b), make_float2(cs[e].x, cs[e].x), __fmul2_rn(make_float2(-b, a), make_float2(cs[e].y, cs[e].y)));
+                            f[c][2 * e] = y.x; f[c][2 * e + 1] = y.y;
+                        }
                     }
+                    x[u].c[c].set(f[c]);
                 }
-                x[u].set(f);
             }
-            const long long to = tk.out[KIND][at_r[u]];
-            if (live && to >= 0) x[u].store(dst + to + at_h[u] * out.sh);
+            const long long to = tk.out[KIND][x[u].r];
+            if (to >= 0) {
+                T* into = dst + (to + x[u].h * out.sh);
+                if (live[0]) x[u].c[0].store(into);
+                if (live[1]) x[u].c[1].store(into + LANES * 8);
+            }
         }
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) { x[u] = nx[u]; at_r[u] = nr[u]; at_h[u] = nh[u]; }
+        for (int u = 0; u < kAhead; ++u) x[u] = next[u];
     }
 }
 
 // blockIdx.x: tokens, blockIdx.y: a share of the heads of q, k and v together
 template <typename T, int LANES>
-__global__ void __launch_bounds__(kThreads, 4) qk_norm_rope_kernel(QkNormRopeParams p, int tokens_per_cta, int heads_per_cta, int heads) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 2) qk_norm_rope_kernel(QkNormRopeParams p, int tokens_per_cta, int heads_per_cta, int heads) {
     __shared__ Tokens tk;
     const int half = p.D / 2;
     const int total = p.B * p.T;
@@ -178,10 +220,9 @@ template <typename T, int LANES>
 int launch_t(cudaStream_t s, const QkNormRopeParams& p) {
     const int heads = (p.q.ptr ? p.Hq : 0) + (p.k.ptr ? p.Hkv : 0) + (p.v.ptr ? p.Hkv : 0);
     const long long total = static_cast<long long>(p.B) * p.T;
-    // Tokens per CTA: 16 where that leaves four rounds of four CTAs per SM (65536 tokens of 32 + 8 heads of 128: 262 us, with 8 273), 8 else (8191 tokens:
-    // 39.7 us, with 16 44.5), fewer where there are not two CTAs per SM.
-    int tokens = (total + 15) / 16 >= 4 * 592 ? 16 : 8;
-    while (tokens > 1 && (total + tokens - 1) / tokens < 296) tokens >>= 1;
+    // One round of the CTAs that fit (four per SM) as long as a CTA's share is at most 16 tokens, and then rounds of that.
+    const long long fit = 4LL * device_sm_count();
+    const int tokens = static_cast<int>(std::min<long long>(kMaxTokens, (total + fit - 1) / fit));
     const long long blocks = (total + tokens - 1) / tokens;
     long long shares = (296 + blocks - 1) / blocks;
     if (shares > heads) shares = heads;
@@ -195,8 +236,8 @@ int launch_t(cudaStream_t s, const QkNormRopeParams& p) {
 
 template <typename T>
 int launch_d(cudaStream_t s, const QkNormRopeParams& p) {
-    const int n = p.D / 8;
-    return n <= 1 ? launch_t<T, 1>(s, p) : n <= 2 ? launch_t<T, 2>(s, p) : n <= 4 ? launch_t<T, 4>(s, p) : n <= 8 ? launch_t<T, 8>(s, p) : launch_t<T, 16>(s, p);
+    const int n = (p.D + 15) / 16;
+    return n <= 1 ? launch_t<T, 1>(s, p) : n <= 2 ? launch_t<T, 2>(s, p) : n <= 4 ? launch_t<T, 4>(s, p) : launch_t<T, 8>(s, p);
 }
 
 }  // namespace
