@@ -297,7 +297,9 @@ __global__ void __launch_bounds__(kThreads, kMinCtas) decode_kv4_kernel(DecodeKv
                 const float2 f = Elem<T>::unpack2(u[i]);
                 x[2 * i] = f.x; x[2 * i + 1] = f.y;
             }
-            new_word = encode8(x, 1.0f / (value ? p.cache.v_unit : p.cache.k_unit), 0xFu << (lane & 28), new_scale);
+            uint32_t got[1];
+            encode<8>(x, 1.0f / (value ? p.cache.v_unit : p.cache.k_unit), 0xFu << (lane & 28), got, new_scale);
+            new_word = got[0];
             if (share == 0) {
                 const long long row = b * p.cache.stride_b + h * p.cache.stride_h + st.len;
                 reinterpret_cast<uint32_t*>(value ? p.cache.v_codes : p.cache.k_codes)[row * (D / 8) + w] = new_word;

@@ -18,13 +18,14 @@ __device__ __forceinline__ float scale_value(uint8_t s) {
     return __half2float(__half(__nv_cvt_fp8_to_halfraw(s, __NV_E4M3)));
 }
 
-// the code word of 8 elements x * back (a power of two) and the scale byte of their group; `lanes`: the 4 threads of the group
-__device__ __forceinline__ uint32_t encode8(float (&x)[8], float back, unsigned lanes, uint8_t& scale) {
+// the code words of N elements x * back (a power of two) and the scale byte of their group; `lanes`: the 32 / N neighbouring threads that have the group
+template <int N>
+__device__ __forceinline__ void encode(float (&x)[N], float back, unsigned lanes, uint32_t (&words)[N / 8], uint8_t& scale) {
     float m = 0.f;                          // a NaN stays one
 #pragma unroll
-    for (int i = 0; i < 8; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(x[i])));
+    for (int i = 0; i < N; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(x[i])));
 #pragma unroll
-    for (int o = 1; o <= 2; o <<= 1) {
+    for (int o = 1; o < kKv4Group / N; o <<= 1) {
         const float other = __shfl_xor_sync(lanes, m, o);
         asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(other));
     }
@@ -39,13 +40,15 @@ __device__ __forceinline__ uint32_t encode8(float (&x)[8], float back, unsigned 
     if (m * r >= 7.5f) {                    // the largest scale, or one of the few small ones that lie far below a seventh: codes end at 7
         const float most = 7.0f * s / back;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = fminf(fmaxf(x[i], -most), most);
+        for (int i = 0; i < N; ++i) x[i] = fminf(fmaxf(x[i], -most), most);
     }
     r *= back;
-    uint32_t word = 0x88888888u;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) word += static_cast<uint32_t>(static_cast<int>(fmaf(x[i], r, copysignf(0.5f, x[i])))) << (4 * i);
-    return word;
+    for (int w = 0; w < N / 8; ++w) {
+        words[w] = 0x88888888u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) words[w] += static_cast<uint32_t>(static_cast<int>(fmaf(x[8 * w + i], r, copysignf(0.5f, x[8 * w + i])))) << (4 * i);
+    }
 }
 
 }  // namespace vb200

@@ -1,6 +1,6 @@
 // Rows of a 4-bit key / value cache: rounding 16-bit rows into it, and reading back what it stands for.
 //
-// What bounds it: HBM.  A thread takes 8 elements of a row (16 bytes, and one 32-bit word of codes), 4 threads share a scale.  A CTA has the places of a few tokens at hand, and each thread several rows on their way.
+// What bounds it: HBM.  A thread takes 16 elements of a row, two threads share a scale.  A CTA has the places of a few tokens at hand, and each thread several rows on their way.
 #include "hybrid.cuh"
 #include "kv4.cuh"
 
@@ -11,13 +11,14 @@ namespace vb200 {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxTokens = 16;             // per CTA
-constexpr int kAhead = 4;                  // rows of a thread at once
+constexpr int kMaxTokens = 32;             // per CTA
+constexpr int kMinCtas = 4;              // per SM, of both kinds
+constexpr int kAhead = 2;                  // rows of a thread at once
 
 // blockIdx.x: tokens; blockIdx.y: k or v.  WRITE: 16-bit rows into the cache; else the other way.
 template <typename T, int D, bool WRITE>
-__global__ void __launch_bounds__(kThreads) kv4_rows_kernel(Kv4RowsParams p, int tokens_per_cta) {
-    constexpr int kLanes = D / 8, kRows = kThreads / kLanes;
+__global__ void __launch_bounds__(kThreads, kMinCtas) kv4_rows_kernel(Kv4RowsParams p, int tokens_per_cta) {
+    constexpr int kLanes = D / 16, kRows = kThreads / kLanes;
     __shared__ long long at[kMaxTokens], row_of[kMaxTokens];                 // of a token, without the head: elements of k or v, and row of the cache (-1: left out)
     const bool value = blockIdx.y != 0;
     const View4& view = value ? p.v : p.k;
@@ -31,32 +32,33 @@ __global__ void __launch_bounds__(kThreads) kv4_rows_kernel(Kv4RowsParams p, int
     }
     __syncthreads();
     T* rows16 = static_cast<T*>(view.ptr);
-    uint32_t* codes = reinterpret_cast<uint32_t*>(value ? p.cache.v_codes : p.cache.k_codes);
+    uint2* codes = reinterpret_cast<uint2*>(value ? p.cache.v_codes : p.cache.k_codes);
     uint8_t* scales = value ? p.cache.v_scales : p.cache.k_scales;
-    const float unit = value ? p.cache.v_unit : p.cache.k_unit;
+    const float unit = value ? p.cache.v_unit : p.cache.k_unit, back = 1.0f / unit;
     const int w = threadIdx.x % kLanes, slot = threadIdx.x / kLanes;
-    const unsigned group = 0xFu << ((threadIdx.x & 31) & ~3);                // the threads that share this one's scale
+    const unsigned group = 3u << ((threadIdx.x & 31) & ~1);                 // the threads that share this one's scale
     // token and head of the next row, tokens first (a head's rows of the cache lie next to each other); then kRows on
     int h = slot / n_tok, r = slot - h * n_tok;
     const int step_h = kRows / n_tok, step_r = kRows - step_h * n_tok, n = n_tok * p.H;
     for (int j0 = slot; j0 < n; j0 += kAhead * kRows) {
-        uint4 raw[kAhead];
-        uint32_t word[kAhead];
+        uint4 raw[kAhead][2];
+        uint2 word[kAhead];
         uint8_t scale[kAhead];
         long long from[kAhead], row[kAhead];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
             row[u] = -1;
             if (j0 + u * kRows < n) {
-                from[u] = at[r] + h * view.sh + w * 8;
+                from[u] = at[r] + h * view.sh + w * 16;
                 row[u] = row_of[r];
                 if (row[u] >= 0) {                                           // the same for the threads of a row
                     row[u] += h * p.cache.stride_h;
                     if (WRITE) {
-                        raw[u] = *reinterpret_cast<const uint4*>(rows16 + from[u]);
+                        const uint4* x = reinterpret_cast<const uint4*>(rows16 + from[u]);
+                        raw[u][0] = x[0]; raw[u][1] = x[1];
                     } else {
                         word[u] = codes[row[u] * kLanes + w];
-                        scale[u] = scales[row[u] * (D / kKv4Group) + w / 4];
+                        scale[u] = scales[row[u] * (D / kKv4Group) + w / 2];
                     }
                 }
             }
@@ -67,25 +69,35 @@ __global__ void __launch_bounds__(kThreads) kv4_rows_kernel(Kv4RowsParams p, int
         for (int u = 0; u < kAhead; ++u) {
             if (row[u] < 0) continue;
             if (WRITE) {
-                const uint32_t x2[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-                float x[8];
+                float x[16];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float2 f = Elem<T>::unpack2(x2[e]);
-                    x[2 * e] = f.x; x[2 * e + 1] = f.y;
+                for (int c = 0; c < 2; ++c) {
+                    const uint32_t x2[4] = {raw[u][c].x, raw[u][c].y, raw[u][c].z, raw[u][c].w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 f = Elem<T>::unpack2(x2[e]);
+                        x[8 * c + 2 * e] = f.x; x[8 * c + 2 * e + 1] = f.y;
+                    }
                 }
-                codes[row[u] * kLanes + w] = encode8(x, 1.0f / unit, group, scale[u]);
-                if ((w & 3) == 0) scales[row[u] * (D / kKv4Group) + w / 4] = scale[u];
+                uint32_t got[2];
+                encode<16>(x, back, group, got, scale[u]);
+                codes[row[u] * kLanes + w] = make_uint2(got[0], got[1]);
+                if ((w & 1) == 0) scales[row[u] * (D / kKv4Group) + w / 2] = scale[u];
             } else {
                 const float s = scale_value(scale[u]) * unit;
-                uint32_t x2[4];
+                uint4* to = reinterpret_cast<uint4*>(rows16 + from[u]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    // 2^23 + n is the float of the bits 0x4B000000 | n
-                    const float lo = __uint_as_float(0x4B000000u | ((word[u] >> (8 * e)) & 15)) - 8388616.0f, hi = __uint_as_float(0x4B000000u | ((word[u] >> (8 * e + 4)) & 15)) - 8388616.0f;
-                    x2[e] = Elem<T>::pack2(lo * s, hi * s);
+                for (int c = 0; c < 2; ++c) {
+                    const uint32_t code = c ? word[u].y : word[u].x;
+                    uint32_t x2[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        // 2^23 + n is the float of the bits 0x4B000000 | n
+                        const float lo = __uint_as_float(0x4B000000u | ((code >> (8 * e)) & 15)) - 8388616.0f, hi = __uint_as_float(0x4B000000u | ((code >> (8 * e + 4)) & 15)) - 8388616.0f;
+                        x2[e] = Elem<T>::pack2(lo * s, hi * s);
+                    }
+                    to[c] = make_uint4(x2[0], x2[1], x2[2], x2[3]);
                 }
-                *reinterpret_cast<uint4*>(rows16 + from[u]) = make_uint4(x2[0], x2[1], x2[2], x2[3]);
             }
         }
     }
@@ -93,7 +105,7 @@ __global__ void __launch_bounds__(kThreads) kv4_rows_kernel(Kv4RowsParams p, int
 
 template <typename T, int D, bool WRITE>
 int launch_t(cudaStream_t s, const Kv4RowsParams& p) {
-    const long long total = static_cast<long long>(p.B) * p.T, fit = 4LL * device_sm_count();
+    const long long total = static_cast<long long>(p.B) * p.T, fit = kMinCtas / 2 * static_cast<long long>(device_sm_count());
     const int tokens = static_cast<int>(std::min<long long>(kMaxTokens, (total + fit - 1) / fit));
     kv4_rows_kernel<T, D, WRITE><<<dim3(static_cast<unsigned>((total + tokens - 1) / tokens), 2), kThreads, 0, s>>>(p, tokens);
     note_launch();
