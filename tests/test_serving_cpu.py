@@ -40,6 +40,18 @@ def test_structs_match_the_header(serving, tmp_path):
     for _, cls in pairs:
         want += [C.sizeof(cls)] + [getattr(cls, f[0]).offset for f in cls._fields_]
     assert got == want
+    # the binding's packings are these structs
+    for packing, cls in ((serving._NORM, serving.QkNormRopeArgs), (serving._PACKED, serving.PackedArgs), (serving._KV4_ROWS, serving.Kv4RowsArgs), (serving._DECODE, serving.DecodeKv4Args)):
+        n = len(packing.unpack(bytes(packing.size)))
+        a = cls.from_buffer_copy(packing.pack(*range(1, n + 1)))
+        flat = []
+
+        def walk(x):
+            for f in x._fields_:
+                y = getattr(x, f[0])
+                walk(y) if isinstance(y, C.Structure) else flat.append(C.cast(y, C.c_void_p).value if isinstance(y, C._Pointer) else y)
+        walk(a)
+        assert packing.size == C.sizeof(cls) and flat == list(range(1, n + 1)), cls
 
 
 def view(capi, H, S, D, ptr=P):

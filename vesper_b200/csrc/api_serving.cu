@@ -27,6 +27,18 @@ vb200_tensor4 used(vb200_tensor4 t, int64_t B, int64_t H, int64_t S) {
     return t;
 }
 
+// f / (2 pi) as a fraction of 2^64, whole turns dropped: f = m * 2^e with a whole m of 24 bits, times 2^100 / (2 pi) as a whole number
+unsigned long long turn_fraction(float f) {
+    int e = 0;
+    const long long m = static_cast<long long>(std::frexp(std::fabs(f), &e) * 16777216.0f);
+    e -= 24;
+    constexpr unsigned __int128 kInverse = (static_cast<unsigned __int128>(0x28be60db9ULL) << 64) | 0x391054a7f09d5f47ULL;
+    const unsigned __int128 x = kInverse * static_cast<unsigned __int128>(m);
+    const int right = 36 - e;              // x * 2^(e - 100 + 64)
+    const unsigned long long t = right >= 128 || right <= -64 ? 0 : right >= 0 ? static_cast<unsigned long long>(x >> right) : static_cast<unsigned long long>(x) << -right;
+    return f < 0.f ? 0 - t : t;
+}
+
 int check_rows(const vb200_rows& r) {
     if (!r.rows) return r.seq_ids ? set_detail(VB200_ERR_INVALID_ARG, "seq_ids without rows") : VB200_OK;
     if (r.seqs <= 0 || r.cap <= 0) return set_detail(VB200_ERR_INVALID_ARG, "rows: seqs and cap of the cache must be positive");
@@ -192,10 +204,7 @@ int vb200_qk_norm_rope(const vb200_qk_norm_rope_args* a) {
     p.k_weight = a->norm ? a->k_weight : nullptr;
     p.rope = a->rope.enabled; p.start_pos = a->start_pos; p.positions = a->positions;
     if (p.rope)
-        for (int i = 0; i < a->D / 2; ++i) {
-            const long double turns = static_cast<long double>(a->rope.inv_freq_host[i]) / 6.283185307179586476925286766559L;
-            p.turns[i] = static_cast<unsigned long long>((turns - std::floor(turns)) * 18446744073709551616.0L);
-        }
+        for (int i = 0; i < a->D / 2; ++i) p.turns[i] = turn_fraction(a->rope.inv_freq_host[i]);
     p.dst = row_map(a->dst);
     if (int rc = status_or_fail(p.status)) return rc;
     return launch_qk_norm_rope(static_cast<cudaStream_t>(a->stream), p);

@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 from . import capi
 
@@ -52,19 +53,24 @@ def load():
     global _lib
     if _lib is None:
         L = capi.load()
-        L.vb200_qk_norm_rope.argtypes = [C.POINTER(QkNormRopeArgs)]
-        L.vb200_prefill_packed_fwd.argtypes = L.vb200_prefill_packed_workspace_bytes.argtypes = [C.POINTER(PackedArgs)]
-        L.vb200_kv4_append.argtypes = L.vb200_kv4_read.argtypes = [C.POINTER(Kv4RowsArgs)]
-        for name in ("vb200_decode_kv4_fwd", "vb200_decode_kv4_workspace_bytes", "vb200_decode_kv4_workspace_bytes_max"):
-            getattr(L, name).argtypes = [C.POINTER(DecodeKv4Args)]
+        for name in SERVING_EXPORTS:                              # an args struct by reference, or its bytes
+            getattr(L, name).argtypes = [_p]
         for name in ("vb200_prefill_packed_workspace_bytes", "vb200_decode_kv4_workspace_bytes", "vb200_decode_kv4_workspace_bytes_max"):
             getattr(L, name).restype = C.c_size_t
         _lib = L
     return _lib
 
 
+# The args structs as one packing each: filling ctypes structures field by field takes most of a small call's time.
+_VIEW = "P3q"                                                 # vb200_tensor4
+_CACHE = "4P2q4i"                                             # vb200_kv4_cache
+_ROWS = "2P2i"                                                # vb200_rows
+_NORM = struct.Struct("@NiP6i" + 6 * _VIEW + "if2PiPiP" + _ROWS + "0q")
+_PACKED = struct.Struct("@NiP8if" + 4 * _VIEW + "4PN0q")
+_KV4_ROWS = struct.Struct("@NiP5i" + 2 * _VIEW + _CACHE + "i" + "0q" + _ROWS + "0q")
+_DECODE = struct.Struct("@NiP5if" + 4 * _VIEW + "P" + _CACHE + "P4iPN0q")
+_NONE4 = (0, 0, 0, 0)
 _TYPES = {}
-_NONE4 = capi.Tensor4(None, 0, 0, 0)
 
 
 def _code(t):
@@ -97,7 +103,7 @@ def _view(name, t, model, shape):
     s = t.stride()
     if t.shape != shape or t.dtype is not model.dtype or t.get_device() != model.get_device() or s[3] != 1:
         _wrong(name, t, shape, model)
-    return capi.Tensor4(t.data_ptr(), s[0], s[1], s[2])
+    return t.data_ptr(), s[0], s[1], s[2]
 
 
 def _view3(name, t, model, shape):
@@ -105,13 +111,13 @@ def _view3(name, t, model, shape):
     s = t.stride()
     if t.shape != shape or t.dtype is not model.dtype or t.get_device() != model.get_device() or s[2] != 1:
         _wrong(name, t, shape, model)
-    return capi.Tensor4(t.data_ptr(), 0, s[1], s[0])
+    return t.data_ptr(), 0, s[1], s[0]
 
 
 def _whole(name, t, dtype, device, numel):
-    """The address of an array that the kernels read as it lies (None: none)."""
+    """The address of an array that the kernels read as it lies (0: none)."""
     if t is None:
-        return None
+        return 0
     if t.dtype is not dtype or t.get_device() != device or t.numel() != numel or not t.is_contiguous():
         raise ValueError(f"{name}: expected {numel} contiguous {dtype} on device {device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
     return t.data_ptr()
@@ -119,7 +125,7 @@ def _whole(name, t, dtype, device, numel):
 
 def _rows(rows, seqs, device, tokens, n_seqs, cap):
     import torch
-    return Rows(_whole("rows", rows, torch.int32, device, tokens), _whole("seqs", seqs, torch.int32, device, tokens), n_seqs, cap)
+    return _whole("rows", rows, torch.int32, device, tokens), _whole("seqs", seqs, torch.int32, device, tokens), n_seqs, cap
 
 
 def _workspace(workspace, need, t, stream):
@@ -145,7 +151,7 @@ def qk_norm_rope(q, k, v=None, *, eps=None, q_weight=None, k_weight=None, theta=
     k_out = k if k_out is None and not scatter else k_out
     if not scatter and v is not None and v_out is None:
         raise ValueError("qk_norm_rope: v needs v_out")
-    dst, kv_out_shape = Rows(), (B, Hkv, T, D)
+    dst, kv_out_shape = _NONE4, (B, Hkv, T, D)
     if scatter:
         cache = k_out if k_out is not None else v_out
         if cache is None:
@@ -154,24 +160,28 @@ def qk_norm_rope(q, k, v=None, *, eps=None, q_weight=None, k_weight=None, theta=
         dst = _rows(rows, seqs, device, B * T, cache.shape[0], cache.shape[2])
     elif seqs is not None:
         raise ValueError("qk_norm_rope: seqs need rows")
-    views = [_NONE4 if t is None else _view(name, t, some, shape) for name, t, shape in (
-        ("q", q, (B, Hq, T, D)), ("k", k, (B, Hkv, T, D)), ("v", v, (B, Hkv, T, D)), ("q_out", q_out, (B, Hq, T, D)), ("k_out", k_out, kv_out_shape), ("v_out", v_out, kv_out_shape))]
-    qw = kw = None
+    shape_q, shape_kv = (B, Hq, T, D), (B, Hkv, T, D)
+    qw = kw = turned = table = 0
     if eps is not None:
         qw, kw = _whole("q_weight", q_weight, torch.float32, device, D), _whole("k_weight", k_weight, torch.float32, device, D)
-    rope = capi.Rope(0, None)
     if inv_freq is None and theta is not None:
         inv_freq = capi.inv_freq(theta, D)
     if inv_freq is not None:
         if len(inv_freq) != D // 2:
             raise ValueError(f"qk_norm_rope: expected {D // 2} frequencies, got {len(inv_freq)}")
-        if not isinstance(inv_freq, C.Array):
-            import numpy as np
-            inv_freq = (C.c_float * (D // 2)).from_buffer_copy(np.ascontiguousarray(inv_freq, dtype=np.float32))
-        rope = capi.Rope(1, inv_freq)
-    a = QkNormRopeArgs(C.sizeof(QkNormRopeArgs), device, _stream(device, stream), _code(some), B, Hq, Hkv, T, D, *views, int(eps is not None), eps or 0.0, qw, kw, rope, start_pos,
-                       _whole("positions", positions, torch.int32, device, B * T), dst)
-    rc = load().vb200_qk_norm_rope(C.byref(a))
+        numpy = getattr(inv_freq, "__array_interface__", None)
+        if numpy is not None and numpy["typestr"] == "<f4" and numpy["strides"] is None:
+            turned, table = 1, numpy["data"][0]
+        else:
+            if not isinstance(inv_freq, C.Array):
+                inv_freq = (C.c_float * (D // 2))(*[float(x) for x in inv_freq])
+            turned, table = 1, C.addressof(inv_freq)
+    a = _NORM.pack(_NORM.size, device, _stream(device, stream), _code(some), B, Hq, Hkv, T, D,
+                   *(_NONE4 if q is None else _view("q", q, some, shape_q)), *(_NONE4 if k is None else _view("k", k, some, shape_kv)),
+                   *(_NONE4 if v is None else _view("v", v, some, shape_kv)), *(_NONE4 if q_out is None else _view("q_out", q_out, some, shape_q)),
+                   *(_NONE4 if k_out is None else _view("k_out", k_out, some, kv_out_shape)), *(_NONE4 if v_out is None else _view("v_out", v_out, some, kv_out_shape)),
+                   int(eps is not None), eps or 0.0, qw, kw, turned, table, start_pos, _whole("positions", positions, torch.int32, device, B * T), *dst)
+    rc = load().vb200_qk_norm_rope(a)
     if rc:
         capi.check(rc)
     return q_out, k_out, v_out
@@ -195,12 +205,12 @@ def prefill_packed(q, k, v, o=None, lse=None, *, scale, cu_seqlens_q, cu_seqlens
     device, batch = q.get_device(), cu_seqlens_q.numel() - 1
     if cu_seqlens_k is None and tk < tq:
         raise ValueError("prefill_packed: fewer keys than queries need cu_seqlens_k")
-    a = PackedArgs(C.sizeof(PackedArgs), device, _stream(device, stream), _code(q), batch, Hq, Hkv, D, tq, tk, int(causal), scale, _view3("q", q, q, (tq, Hq, D)),
-                   _view3("o", o, q, (tq, Hq, D)), _view3("k", k, q, (tk, Hkv, D)), _view3("v", v, q, (tk, Hkv, D)), _whole("lse", lse, torch.float32, device, tq * Hq),
-                   _whole("cu_seqlens_q", cu_seqlens_q, torch.int32, device, batch + 1), _whole("cu_seqlens_k", cu_seqlens_k, torch.int32, device, batch + 1))
     L = load()
-    a.workspace, a.workspace_bytes = _workspace(workspace, 0 if workspace is not None else L.vb200_prefill_packed_workspace_bytes(C.byref(a)), q, stream)
-    rc = L.vb200_prefill_packed_fwd(C.byref(a))
+    address, size = _workspace(workspace, 0 if workspace is not None else L.vb200_prefill_packed_workspace_bytes(C.byref(_packed_args(q, k, batch))), q, stream)
+    rc = L.vb200_prefill_packed_fwd(_PACKED.pack(
+        _PACKED.size, device, _stream(device, stream), _code(q), batch, Hq, Hkv, D, tq, tk, int(causal), scale, *_view3("q", q, q, (tq, Hq, D)), *_view3("o", o, q, (tq, Hq, D)),
+        *_view3("k", k, q, (tk, Hkv, D)), *_view3("v", v, q, (tk, Hkv, D)), _whole("lse", lse, torch.float32, device, tq * Hq),
+        _whole("cu_seqlens_q", cu_seqlens_q, torch.int32, device, batch + 1), _whole("cu_seqlens_k", cu_seqlens_k, torch.int32, device, batch + 1), address, size))
     if rc:
         capi.check(rc)
     return o
@@ -225,8 +235,9 @@ class Kv4Cache:
             if any(t.shape[d] > 1 and t.stride(d) * row != k_codes.stride(d) * n for d in (0, 1)):
                 raise ValueError("Kv4Cache: codes and scales must have the same strides, in rows")
         self.device = k_codes.get_device()
-        self.view = Kv4CacheView(_ptr(k_codes), _ptr(v_codes), _ptr(k_scales), _ptr(v_scales), k_codes.stride(0) // row, k_codes.stride(1) // row, self.seqs, self.cap,
-                                 k_exponent, v_exponent)
+        fields = (_ptr(k_codes), _ptr(v_codes), _ptr(k_scales), _ptr(v_scales), k_codes.stride(0) // row, k_codes.stride(1) // row, self.seqs, self.cap,
+                  k_exponent, v_exponent)
+        self.view, self._fields = Kv4CacheView(*fields), fields
 
     def _call(self, entry, k, v, start_row, rows, seqs, stream):
         some = k if k is not None else v
@@ -238,9 +249,9 @@ class Kv4Cache:
             raise ValueError(f"Kv4Cache: rows on {some.device}, cache on {self.k_codes.device}")
         if seqs is not None and rows is None:
             raise ValueError("Kv4Cache: seqs need rows")
-        a = Kv4RowsArgs(C.sizeof(Kv4RowsArgs), device, _stream(device, stream), _code(some), B, self.Hkv, T, self.D, _NONE4 if k is None else _view("k", k, some, shape),
-                        _NONE4 if v is None else _view("v", v, some, shape), self.view, start_row, _rows(rows, seqs, device, B * T, self.seqs, self.cap))
-        rc = entry(C.byref(a))
+        rc = entry(_KV4_ROWS.pack(
+            _KV4_ROWS.size, device, _stream(device, stream), _code(some), B, self.Hkv, T, self.D, *(_NONE4 if k is None else _view("k", k, some, shape)),
+            *(_NONE4 if v is None else _view("v", v, some, shape)), *self._fields, start_row, *_rows(rows, seqs, device, B * T, self.seqs, self.cap)))
         if rc:
             capi.check(rc)
 
@@ -272,13 +283,13 @@ def decode_kv4(q, o, cache, *, scale, k_new=None, v_new=None, lse=None, seq_lens
     device, shape, new = q.get_device(), (B, Hq, 1, cache.D), (B, cache.Hkv, 1, cache.D)
     if device != cache.device:
         raise ValueError(f"decode_kv4: q on {q.device}, cache on {cache.k_codes.device}")
-    a = DecodeKv4Args(C.sizeof(DecodeKv4Args), device, _stream(device, stream), _code(q), B, Hq, cache.Hkv, cache.D, scale, _view("q", q, q, shape),
-                      _NONE4 if k_new is None else _view("k_new", k_new, q, new), _NONE4 if v_new is None else _view("v_new", v_new, q, new), _view("o", o, q, shape),
-                      _whole("lse", lse, torch.float32, device, B * Hq), cache.view, _whole("seq_lens", seq_lens, torch.int32, device, B), uniform_len, int(advance_lens),
-                      max_len, num_splits)
     L = load()
-    a.workspace, a.workspace_bytes = _workspace(workspace, 0 if workspace is not None else L.vb200_decode_kv4_workspace_bytes(C.byref(a)), q, stream)
-    rc = L.vb200_decode_kv4_fwd(C.byref(a))
+    address, size = _workspace(workspace, 0 if workspace is not None else L.vb200_decode_kv4_workspace_bytes(C.byref(_decode_args(q, cache, max_len, num_splits))), q, stream)
+    rc = L.vb200_decode_kv4_fwd(_DECODE.pack(
+        _DECODE.size, device, _stream(device, stream), _code(q), B, Hq, cache.Hkv, cache.D, scale, *_view("q", q, q, shape),
+        *(_NONE4 if k_new is None else _view("k_new", k_new, q, new)), *(_NONE4 if v_new is None else _view("v_new", v_new, q, new)), *_view("o", o, q, shape),
+        _whole("lse", lse, torch.float32, device, B * Hq), *cache._fields, _whole("seq_lens", seq_lens, torch.int32, device, B), uniform_len, int(advance_lens), max_len, num_splits,
+        address, size))
     if rc:
         capi.check(rc)
     return o
