@@ -494,11 +494,10 @@ __global__ void __launch_bounds__(kThreads, kMinCtas) decode_kv4_kernel(DecodeKv
 
 // Merges the parts of a query head whose unit several CTAs had: o = sum_i o_i l_i 2^(m_i - m) / sum_i l_i 2^(m_i - m); writes the zeros of sequences without rows
 // and stores the advanced length.  Every CTA and unit that meet have a record of their own at CTA + unit: along the row of tiles both only grow, so no
-// two meetings share one, and a unit's parts lie one behind the other.  512 threads: 512 / D groups of parts.
-constexpr int kCombineThreads = 512;
-template <typename T, int D>
-__global__ void __launch_bounds__(kCombineThreads) decode_kv4_combine_kernel(DecodeKv4Params p, int head_shares) {
-    constexpr int kGroups = kCombineThreads / D;
+// two meetings share one, and a unit's parts lie one behind the other.  THREADS / D groups of parts.
+template <typename T, int D, int THREADS>
+__global__ void __launch_bounds__(THREADS) decode_kv4_combine_kernel(DecodeKv4Params p, int head_shares) {
+    constexpr int kGroups = THREADS / D;
     __shared__ float sum_of[kGroups][D], l_of[kGroups];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -584,7 +583,11 @@ int launch_t(cudaStream_t s, const DecodeKv4Params& p) {
     profile_mark_end(s);
     note_launch();
     if (!p.per_unit || p.advance_lens) {
-        VB200_CUDA_TRY(launch_dependent(decode_kv4_combine_kernel<T, D>, dim3(p.Hq, p.B), kCombineThreads, 0, s, p, shares));
+        // Many parts to a unit: 512 threads a head (131072 keys of one sequence, 37 parts: 47.0 us, with 128 threads 49.9); few parts, but many heads: 128
+        // (32 sequences of 1024-8192 keys: 54.0 us, with 512 threads 57.6).
+        const dim3 grid(p.Hq, p.B);
+        if (p.ctas >= 8LL * p.B * p.Hkv * shares) VB200_CUDA_TRY(launch_dependent(decode_kv4_combine_kernel<T, D, 512>, grid, 512, 0, s, p, shares));
+        else VB200_CUDA_TRY(launch_dependent(decode_kv4_combine_kernel<T, D, 128>, grid, 128, 0, s, p, shares));
         note_launch();
     }
     return VB200_OK;
