@@ -30,7 +30,8 @@ typedef struct vb200_rows {
  * For every head of q and k, y = x / sqrt(mean(x^2) + eps) * weight over its D elements (norm == 0: y = x), then the pairs (y[2i], y[2i+1]) are turned
  * by the angle position * inv_freq[i] (rope.enabled == 0: not turned); all in fp32, rounded once.  The product position * inv_freq[i] is not rounded
  * to fp32 as apply_rotary_emb does it (a thousandth of a radian at position 16384): rotate the queries and the keys of one cache with one of the two.
- * Outputs stand like the inputs (and may be the same memory: q_out == q with the same strides; overlapping otherwise is not allowed), or, with
+ * Outputs stand like the inputs (and may be the same memory: q_out == q with the same strides; overlapping otherwise is not allowed, and neither are negative
+ * strides), or, with
  * dst.rows, k_out and v_out are [dst.seqs, Hkv, dst.cap, D] caches and token (b, t) is written where `dst` says.
  * Any of q, k, v may be left out (ptr null together with its output's); v is copied, which needs an output of its own. */
 typedef struct vb200_qk_norm_rope_args {
@@ -58,9 +59,10 @@ int vb200_qk_norm_rope(const vb200_qk_norm_rope_args* a);
  * values the tokens [cu_seqlens_k[i], cu_seqlens_k[i+1]) of k and v (null: the same as cu_seqlens_q).  The lengths stay on the device.  Causal aligns
  * the last query with the last key: query i of n_q sees key j of n_k iff j <= n_k - n_q + i.  A query that sees no key gets zeros and an lse of
  * -infinity.  Tokens behind the last sequence are neither read (k, v) nor written (o, lse).  The running sums are fp32; the weights are rounded to
- * `dtype` for their product with v.  A non-finite value reaches every query of its sequence whose block of 128 keys holds it, like in vb200_prefill_fwd;
- * it never reaches another sequence.
- * The offsets have to ascend from 0 and end within the tokens given: sequences that do not are left out. */
+ * `dtype` for their product with v.  A non-finite value reaches every query of its sequence that sees a key of its block of at most 112 keys (a weight of zero
+ * times infinity is NaN), as in vb200_prefill_fwd; it never reaches another sequence.
+ * The offsets have to ascend and to stay within the tokens given.  A sequence whose own two do not is left out; nothing outside the tensors is read or
+ * written whatever they are. */
 typedef struct vb200_prefill_packed_args {
     size_t struct_size;
     int32_t device;
@@ -70,7 +72,7 @@ typedef struct vb200_prefill_packed_args {
     int32_t total_q, total_k;    /* tokens of q / o and of k / v */
     int32_t causal;
     float scale;
-    vb200_tensor4 q, o;          /* [total_q, Hq, D]: stride_s between tokens, stride_h between heads (stride_b is not looked at) */
+    vb200_tensor4 q, o;          /* [total_q, Hq, D]: stride_s between tokens, stride_h between heads, both positive (stride_b is not looked at) */
     vb200_tensor4 k, v;          /* [total_k, Hkv, D] */
     float* lse;                  /* [Hq, total_q] contiguous fp32, nullable */
     const int32_t* cu_seqlens_q; /* device [batch + 1] */

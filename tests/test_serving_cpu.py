@@ -105,7 +105,7 @@ def packed_args(serving, **kw):
 @pytest.mark.parametrize("status, change", [
     (-1, dict(struct_size=8)), (-2, dict(dtype=0)), (-2, dict(D=96)), (-2, dict(D=256)), (-1, dict(batch=0)), (-1, dict(batch=70000)), (-1, dict(Hkv=3)), (-1, dict(Hkv=0)),
     (-1, dict(total_q=0)), (-1, dict(total_k=-1)), (-1, dict(cu_seqlens_q=None)), (-4, dict(workspace=None)), (-4, dict(workspace_bytes=16)), (-3, dict(workspace=P + 16)),
-    (-1, dict(total_q=2 ** 30))])
+    (-1, dict(total_q=2 ** 30)), (-1, dict(batch=65536, Hq=65536, Hkv=65536))])
 def test_packed_refuses(serving, status, change):
     assert serving.load().vb200_prefill_packed_fwd(C.byref(packed_args(serving, **change))) == status
 
@@ -117,6 +117,7 @@ def test_packed_refuses_views(serving):
         assert call(**{name: capi.Tensor4(None, 0, 128, 1024)}) == -1
         assert call(**{name: capi.Tensor4(P + 8, 0, 128, 1024)}) == -3
         assert call(**{name: capi.Tensor4(P, 0, 128, 1028)}) == -3
+        assert call(**{name: capi.Tensor4(P, 0, 0, 1024)}) == -2 and call(**{name: capi.Tensor4(P, 0, 128, 0)}) == -2
     assert serving.load().vb200_prefill_packed_workspace_bytes(C.byref(packed_args(serving, Hkv=3))) == 0
     assert serving.load().vb200_prefill_packed_workspace_bytes(C.byref(packed_args(serving))) > 0
 

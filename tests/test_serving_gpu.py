@@ -170,12 +170,13 @@ def check_packed(q, k, v, o, lse, lens_q, lens_k, scale, causal):
         x += nk
 
 
-LENGTHS = [[1], [128], [5, 0, 130, 1], [129, 127, 300, 64, 65], [31, 32, 33, 16, 17, 8, 9], [700, 3, 513], [0, 2, 0], list(range(1, 41))]
+LENGTHS = [[1], [128], [79, 80, 81], [111, 112, 113, 15], [159, 160, 161, 223, 224, 225], [5, 0, 130, 1], [129, 127, 300, 64, 65], [31, 32, 33, 16, 17, 8, 9], [700, 3, 513], [0, 2, 0], list(range(1, 41))]
 
 
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("lens", LENGTHS)
-@pytest.mark.parametrize("Hq, Hkv, D, dtype", [(8, 2, 128, torch.bfloat16), (4, 4, 64, torch.float16), (6, 2, 128, torch.float16), (8, 1, 64, torch.bfloat16), (3, 3, 128, torch.bfloat16)])
+@pytest.mark.parametrize("Hq, Hkv, D, dtype", [(8, 2, 128, torch.bfloat16), (4, 4, 64, torch.float16), (6, 2, 128, torch.float16), (8, 1, 64, torch.bfloat16), (3, 3, 128, torch.bfloat16), (80, 80, 64, torch.bfloat16),
+                                               (320, 80, 128, torch.float16)])
 def test_packed(S, lens, causal, Hq, Hkv, D, dtype):
     g = rng(len(lens) * 7 + Hq)
     (q, k, v), cu, _ = packed_case(g, lens, lens, Hq, Hkv, D, dtype)
@@ -208,6 +209,19 @@ def test_packed_portions(S, lens_q, lens_k, causal, Hq, Hkv, D):
     check_packed(q, k, v, o, lse, lens_q, lens_k, D ** -0.5, causal)
     if sum(lens_q) == 0:
         assert bool((o == 9.0).all()) and bool((lse == 9.0).all())
+
+
+@pytest.mark.parametrize("Hq, Hkv, D", [(8, 2, 64), (40, 40, 64)])
+def test_packed_many_sequences(S, Hq, Hkv, D):
+    """More sequences than the planning block keeps at hand, most of them of a few tokens, some empty."""
+    r = np.random.RandomState(Hq)
+    lens = [int(x) for x in r.randint(0, 7, 1500)]
+    lens[700], lens[1499] = 400, 90
+    g = rng(Hq)
+    (q, k, v), cu, _ = packed_case(g, lens, lens, Hq, Hkv, D, torch.bfloat16)
+    o, lse = torch.empty_like(q), torch.empty(Hq, q.shape[0], device=DEV)
+    S.prefill_packed(q, k, v, o, lse, scale=0.125, cu_seqlens_q=cu)
+    check_packed(q, k, v, o, lse, lens, lens, 0.125, True)
 
 
 def test_packed_no_keys_at_all(S):
@@ -266,6 +280,12 @@ def test_packed_refuses_offsets_on_the_device(S):
             if (a, b) != (0, 30):                                          # (0, 30) and (20, 60) share tokens here: whichever came last stands
                 assert torch.equal(o[max(a, 30):b], want[max(a, 30) - a:])
         assert bool((o[~touched] == 3.0).all())
+    # the same tokens named over and over: more items than the tokens make, and nothing outside them
+    q2, k2, v2 = (x.repeat(1, 40, 1).contiguous() for x in (q, k, v))
+    o = torch.full_like(q2, 3.0)
+    S.prefill_packed(q2, k2, v2, o, scale=0.125, cu_seqlens_q=int32([0, 100] * 300))
+    want = S.prefill_packed(q2, k2, v2, scale=0.125, cu_seqlens_q=int32([0, 100]))
+    assert bool(((o == want) | (o == 3.0)).all())
 
 
 def test_packed_large_scores(S):

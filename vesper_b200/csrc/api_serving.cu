@@ -144,7 +144,7 @@ int check_packed(const vb200_prefill_packed_args* a) {
     if (a->Hq % a->Hkv != 0) return set_detail(VB200_ERR_INVALID_ARG, "Hq must be divisible by Hkv");
     if (!a->q.ptr || !a->o.ptr || (a->total_k > 0 && (!a->k.ptr || !a->v.ptr))) return set_detail(VB200_ERR_INVALID_ARG, "q, k, v, o must be non-null");
     if (!a->cu_seqlens_q) return set_detail(VB200_ERR_INVALID_ARG, "cu_seqlens_q must be non-null");
-    if (!countable(1, a->total_q, a->Hq) || a->batch > 65536) return set_detail(VB200_ERR_INVALID_ARG, "packed attention: at most 2^31 - 1 (token, head) pairs and 65536 sequences");
+    if (!countable(1, static_cast<int64_t>(a->total_q) + a->batch, a->Hq) || a->batch > 65536) return set_detail(VB200_ERR_INVALID_ARG, "packed attention: at most 2^31 - 1 (token, head) pairs and 65536 sequences");
     auto dense = [](const vb200_tensor4& t, int H, int tokens) { return (H == 1 || t.stride_h > 0) && (tokens <= 1 || t.stride_s > 0); };
     if (!dense(a->q, a->Hq, a->total_q) || !dense(a->o, a->Hq, a->total_q) || !dense(a->k, a->Hkv, a->total_k) || !dense(a->v, a->Hkv, a->total_k))
         return set_detail(VB200_ERR_UNSUPPORTED, "packed attention: strides must be positive (no broadcast heads or tokens)");

@@ -104,7 +104,7 @@ constexpr int kAtHand = 1024;              // sequences that the planning block 
 
 __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedParams p, int tile_tokens, int max_items, Plan* plan, Item* items, int* first_in_memory) {
     __shared__ int hist[kBins];
-    __shared__ int warp_sum[32];
+    __shared__ long long warp_sum[32];
     __shared__ int first_at_hand[kAtHand + 1];
     __shared__ Sequence at_hand[kAtHand];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, pair = 2 * tile_tokens;
@@ -114,46 +114,47 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedParams 
     hist[tid] = 0;
     // first item of each sequence: every thread a piece of the sequences, then a sum over the threads before it
     const int per = (p.batch + kPlanThreads - 1) / kPlanThreads, i0 = min(tid * per, p.batch), i1 = min(i0 + per, p.batch);
-    int mine = 0;
+    long long mine = 0;                                  // (offsets that do not ascend may name more tokens than there are)
     for (int i = i0; i < i1; ++i) {
         const Sequence s = sequence_of(p, i);
         if (small) at_hand[i] = s;
         mine += (s.nq + pair - 1) / pair;
     }
     auto sequence = [&](int i) { return small ? at_hand[i] : sequence_of(p, i); };
-    auto scan = [&](int x) {                             // inclusive, over the block
+    auto scan = [&](long long x) {                       // inclusive, over the block
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+            const long long y = __shfl_up_sync(0xFFFFFFFFu, x, o);
             if (lane >= o) x += y;
         }
         if (lane == 31) warp_sum[warp] = x;
         __syncthreads();
         if (warp == 0) {
-            int y = warp_sum[lane];
+            long long y = warp_sum[lane];
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int z = __shfl_up_sync(0xFFFFFFFFu, y, o);
+                const long long z = __shfl_up_sync(0xFFFFFFFFu, y, o);
                 if (lane >= o) y += z;
             }
             warp_sum[lane] = y;
         }
         __syncthreads();
-        const int before = warp > 0 ? warp_sum[warp - 1] : 0;
+        const long long before = warp > 0 ? warp_sum[warp - 1] : 0;
         __syncthreads();
         return x + before;
     };
-    int next = scan(mine) - mine;
+    long long next = scan(mine) - mine;
     for (int i = i0; i < i1; ++i) {
-        first_item[i] = next;
+        first_item[i] = static_cast<int>(min(next, static_cast<long long>(max_items)));
         next += (sequence(i).nq + pair - 1) / pair;
     }
     if (i1 == p.batch && i0 < i1) {
-        first_item[p.batch] = next;
-        plan->items = min(next, max_items);              // (offsets in order leave no more than max_items)
+        const int n = static_cast<int>(min(next, static_cast<long long>(max_items)));      // (offsets in order leave no more than max_items)
+        first_item[p.batch] = n;
+        plan->items = n;
     }
     __syncthreads();
-    const int n = min(first_item[p.batch], max_items);
+    const int n = first_item[p.batch];
     auto item_at = [&](int idx) {
         int lo = 0, hi = p.batch;                        // the last sequence whose first item is at or before idx
         while (hi - lo > 1) {
@@ -168,8 +169,7 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedParams 
     }
     __syncthreads();
     const int count = hist[tid];
-    const int at = scan(count) - count;
-    hist[tid] = at;
+    hist[tid] = static_cast<int>(scan(count)) - count;
     __syncthreads();
     for (int idx = tid; idx < n; idx += kPlanThreads) {  // (the order within a bin is free: results do not depend on it)
         const Item w = item_at(idx);
