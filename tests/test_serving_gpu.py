@@ -224,6 +224,46 @@ def test_packed_many_sequences(S, Hq, Hkv, D):
     check_packed(q, k, v, o, lse, lens, lens, 0.125, True)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("Hq, Hkv, D, dtype", [(16, 16, 64, torch.float16), (16, 16, 128, torch.bfloat16), (32, 8, 128, torch.bfloat16), (12, 4, 64, torch.bfloat16), (64, 2, 128, torch.float16),
+                                               (15, 15, 64, torch.bfloat16)])
+def test_packed_short_sequences(S, Hq, Hkv, D, dtype, many, causal):
+    """Sequences of less than a tile, most of them, of which two blocks of heads are computed together (an odd number of blocks: not); prefixes, fewer keys than
+    tokens, none, and NaN behind the last."""
+    rep = Hq // Hkv
+    fold = 16 if rep == 32 else 4 if rep == 4 else 1
+    tile = 128 // fold
+    n = 150 * fold // Hq + 2 if not many else 700 * fold // Hq + 3
+    r = np.random.RandomState(Hq + D)
+    lens_q = [int(x) for x in r.randint(0, tile + 1, n)]
+    lens_q[0], lens_q[1] = 2 * tile + 3, 1
+    lens_k = [a + int(r.choice([0, 0, 3, 117, 400])) if i % 7 else a // 2 for i, a in enumerate(lens_q)]
+    lens_k[-1] = 0 if lens_q[-1] else 5
+    g = rng(Hq)
+    (q, k, v), cu_q, cu_k = packed_case(g, lens_q, lens_k, Hq, Hkv, D, dtype)
+    k, v = (torch.cat([x, torch.full_like(x[:40], math.nan)]) for x in (k, v))
+    o, lse = torch.full_like(q, 9.0), torch.full((Hq, q.shape[0]), 9.0, device=DEV)
+    S.prefill_packed(q, k, v, o, lse, scale=D ** -0.5, cu_seqlens_q=cu_q, cu_seqlens_k=cu_k, causal=causal)
+    check_packed(q, k, v, o, lse, lens_q, lens_k, D ** -0.5, causal)
+    again = torch.zeros_like(o)
+    S.prefill_packed(q, k, v, again, scale=D ** -0.5, cu_seqlens_q=cu_q, cu_seqlens_k=cu_k, causal=causal)
+    assert torch.equal(o, again)
+
+
+def test_packed_workspace_of_the_largest_call(S):
+    """A workspace made for a batch's most tokens serves every smaller number."""
+    Hq, Hkv, D, n = 16, 16, 64, 40
+    q, k = torch.empty(n * 300, Hq, D, dtype=torch.bfloat16, device=DEV), torch.empty(n * 300, Hkv, D, dtype=torch.bfloat16, device=DEV)
+    workspace = S.prefill_packed_workspace(q, k, batch=n)
+    for each in (300, 161, 160, 159, 128, 20, 1):
+        g = rng(each)
+        (q, k, v), cu, _ = packed_case(g, [each] * n, [each] * n, Hq, Hkv, D, torch.bfloat16)
+        o, lse = torch.empty_like(q), torch.empty(Hq, q.shape[0], device=DEV)
+        S.prefill_packed(q, k, v, o, lse, scale=0.125, cu_seqlens_q=cu, workspace=workspace)
+        check_packed(q, k, v, o, lse, [each] * n, [each] * n, 0.125, True)
+
+
 def test_packed_no_keys_at_all(S):
     g = rng(1)
     q = randn(g, 5, 4, 64)
@@ -264,6 +304,23 @@ def test_packed_sequences_do_not_reach_each_other(S):
     v2[60:80] = math.nan
     got = S.prefill_packed(q, k2, v2, scale=0.09, cu_seqlens_q=cu)
     assert torch.equal(got[:60], clean[:60]) and torch.equal(got[137:], clean[137:]) and not torch.isfinite(got[60:137].float()).all()
+
+
+def test_packed_short_sequences_do_not_reach_each_other(S):
+    """The same where two blocks of heads are computed together; and a key head full of NaN and infinities leaves the other heads' bits alone."""
+    g = rng(5)
+    lens = [37, 80, 5] * 14
+    (q, k, v), cu, _ = packed_case(g, lens, lens, 16, 16, 64, torch.bfloat16)
+    clean = S.prefill_packed(q, k, v, scale=0.125, cu_seqlens_q=cu)
+    a, b = sum(lens[:4]), sum(lens[:5])
+    k2, v2 = k.clone(), v.clone()
+    k2[a:b], v2[a:b] = math.nan, math.inf
+    got = S.prefill_packed(q, k2, v2, scale=0.125, cu_seqlens_q=cu)
+    assert torch.equal(got[:a], clean[:a]) and torch.equal(got[b:], clean[b:]) and not torch.isfinite(got[a:b].float()).any()
+    k2, v2 = k.clone(), v.clone()
+    k2[:, 6], v2[:, 6] = math.nan, math.inf
+    got = S.prefill_packed(q, k2, v2, scale=0.125, cu_seqlens_q=cu)
+    assert torch.equal(got[:, :6], clean[:, :6]) and torch.equal(got[:, 7:], clean[:, 7:]) and not torch.isfinite(got[:, 6].float()).any()
 
 
 def test_packed_refuses_offsets_on_the_device(S):

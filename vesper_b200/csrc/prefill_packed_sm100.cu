@@ -5,8 +5,9 @@
 //
 // A tile is 128 rows: 128 / F tokens of one sequence by F heads of one key head's group (F: the power of two of the group, at most 16), row = token * F +
 // head, as one TMA box of q brings them.  Short sequences fill a tile with heads instead of padding, and the rows of a tile see nearly the same keys.  A work
-// item is two tiles of neighbouring tokens that read the same blocks of keys.  The lengths are on the device: a first kernel lists the items with the
-// longest first, then persistent CTAs, one per SM, take them in snake order.
+// item is two tiles of neighbouring tokens that read the same blocks of keys; where the sequences are
+// short, two blocks of heads of the same tokens (two_head_blocks).  The lengths are on the device: a first kernel lists the items with the longest first, then
+// persistent CTAs, one per SM, take them in snake order.
 //   warps 0-3    softmax and epilogue of tile 0, a row per thread (TMEM lane)
 //   warps 4-7    the same for tile 1
 //   warp  8      TMA: q tiles (3 buffers, so that the next item's come while this one computes) and the ring of key and value blocks
@@ -39,7 +40,7 @@ constexpr float kLift = 7.0f;              // which weighs 2^7, so that fp16 wei
 constexpr int kRegSoftmax = 216, kRegOther = 72;
 static_assert(kRegSoftmax * 256 + kRegOther * 128 <= 168 * 384, "register budget");
 
-// Two tiles of neighbouring tokens of a sequence, without the head block: tokens [q0, q0 + tokens), keys [k0, k0 + keys), of which the last that token i
+// Two tiles of a sequence, without the head block: tokens [q0, q0 + tokens), keys [k0, k0 + keys), of which the last that token i
 // sees is `last` + i (causal).
 struct alignas(16) Item {
     int q0, tokens, k0, keys;
@@ -52,18 +53,30 @@ struct Plan {                              // workspace: the header, the items, 
 
 struct Shape {
     int fold, tokens;                      // heads and tokens of a tile
-    int head_blocks;                       // of the model
-    int max_items;                         // without head blocks
+    int dual, item_tokens;                 // whether an item's tiles are two head blocks of the same tokens; tokens of an item
+    int head_blocks;                       // items of the same tokens
+    int max_items, room;                   // without head blocks; what a workspace holds (it does not shrink as tokens are added)
 };
-Shape shape_of(int batch, int Hq, int Hkv, int total_q) {
+Shape shape_of(int batch, int Hq, int Hkv, int total_q, bool dual = false) {
     Shape s;
     const int rep = Hq / Hkv;
     s.fold = 1;
     while (s.fold < 16 && rep % (2 * s.fold) == 0) s.fold *= 2;
     s.tokens = kBlockM / s.fold;
-    s.head_blocks = Hq / s.fold;
-    s.max_items = total_q / (2 * s.tokens) + batch;
+    s.dual = dual;
+    s.item_tokens = dual ? s.tokens : 2 * s.tokens;
+    s.head_blocks = Hq / s.fold / (dual ? 2 : 1);
+    s.max_items = total_q / s.item_tokens + batch;
+    s.room = total_q / s.tokens + batch;
     return s;
+}
+// Sequences of about a tile leave the second tile of an item empty, or nearly: there its tiles are two blocks of heads, which costs keys and values of their own
+// for both.  Lengths are known by their mean alone.  Measured over lengths spread 2- to 16-fold: with head_dim 64 it gains 5 to 27 % at a mean of 0.9 tiles and loses
+// 3 to 11 % at 1.4, with 128 it gains up to 20 % at 0.7 and loses up to 14 % at 0.9 (blocks of keys are twice as large); and always where items of
+// neighbouring tokens already fit the SMs at once, up to 40 %.  (40 sequences of 20-494 tokens, 16 heads of 64: 33.2 us, with tiles of neighbouring tokens 36.3.)
+bool two_head_blocks(const PackedParams& p, const Shape& s) {
+    return s.head_blocks % 2 == 0 && 4ll * p.total_q <= static_cast<int64_t>(p.batch) * s.tokens * (p.D == 64 ? 5 : 3) &&
+           static_cast<int64_t>(p.batch) * s.head_blocks > device_sm_count();
 }
 
 // ---- the list of items, by descending number of keys ----
@@ -84,30 +97,31 @@ __device__ __forceinline__ Sequence sequence_of(const PackedParams& p, int i) {
     return ok ? Sequence{a, b - a, x, y - x} : Sequence{0, 0, 0, 0};
 }
 
-__device__ __forceinline__ Item make_item(const PackedParams& p, const Sequence& s, int r0, int tile_tokens) {
+__device__ __forceinline__ Item make_item(const PackedParams& p, const Shape& shape, const Sequence& s, int r0) {
     Item w;
     w.q0 = s.q0 + r0;
-    w.tokens = min(2 * tile_tokens, s.nq - r0);
+    w.tokens = min(shape.item_tokens, s.nq - r0);
     w.k0 = s.k0;
     w.keys = s.nk;
     w.last = p.causal ? s.nk - s.nq + r0 : s.nk - 1;
     w.pad = 0;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-        const int end = p.causal ? max(0, min(s.nk, w.last + min(w.tokens, (t + 1) * tile_tokens))) : s.nk;
-        w.end[t] = w.tokens > t * tile_tokens ? end : -1;
+        const int first = shape.dual ? 0 : t * shape.tokens;                 // of the tile's tokens
+        const int end = p.causal ? max(0, min(s.nk, w.last + min(w.tokens, first + shape.tokens))) : s.nk;
+        w.end[t] = w.tokens > first ? end : -1;
     }
     return w;
 }
 
 constexpr int kAtHand = 1024;              // sequences that the planning block keeps in shared memory
 
-__global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedParams p, int tile_tokens, int max_items, Plan* plan, Item* items, int* first_in_memory) {
+__global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedParams p, Shape shape, Plan* plan, Item* items, int* first_in_memory) {
     __shared__ int hist[kBins];
     __shared__ long long warp_sum[32];
     __shared__ int first_at_hand[kAtHand + 1];
     __shared__ Sequence at_hand[kAtHand];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, pair = 2 * tile_tokens;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, pair = shape.item_tokens, max_items = shape.max_items;
     const bool small = p.batch <= kAtHand;
     int* first_item = small ? first_at_hand : first_in_memory;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the attention kernel sets itself up meanwhile, and waits for this one
@@ -161,7 +175,7 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedParams 
             const int mid = (lo + hi) / 2;
             if (first_item[mid] <= idx) lo = mid; else hi = mid;
         }
-        return make_item(p, sequence(lo), (idx - first_item[lo]) * pair, tile_tokens);
+        return make_item(p, shape, sequence(lo), (idx - first_item[lo]) * pair);
     };
     for (int idx = tid; idx < n; idx += kPlanThreads) {
         const Item w = item_at(idx);
@@ -251,7 +265,7 @@ __device__ __forceinline__ float2 exp2_fma(float2 x) {
 
 // The item of this CTA where no list is made: found by one warp, 32 sequences at a time.  Returns whether there is one.
 __device__ __forceinline__ bool find_item(const PackedParams& p, const Shape& shape, Item* own) {
-    const int lane = threadIdx.x & 31, pair = 2 * shape.tokens, want = blockIdx.x / shape.head_blocks;
+    const int lane = threadIdx.x & 31, pair = shape.item_tokens, want = blockIdx.x / shape.head_blocks;
     int before = 0;
     for (int i0 = 0; i0 < p.batch; i0 += 32) {
         Sequence s{0, 0, 0, 0};
@@ -265,7 +279,7 @@ __device__ __forceinline__ bool find_item(const PackedParams& p, const Shape& sh
         }
         const unsigned here = __ballot_sync(0xFFFFFFFFu, before + upto > want);
         if (here) {
-            if (lane == __ffs(here) - 1) *own = make_item(p, s, (want - before - (upto - n)) * pair, shape.tokens);
+            if (lane == __ffs(here) - 1) *own = make_item(p, shape, s, (want - before - (upto - n)) * pair);
             return true;
         }
         before += __shfl_sync(0xFFFFFFFFu, upto, 31);
@@ -273,8 +287,9 @@ __device__ __forceinline__ bool find_item(const PackedParams& p, const Shape& sh
     return false;
 }
 
-// kList: the items come from the list; else every CTA has at most one, which it finds itself.  (A template parameter: with a branch on it head_dim 64 lost 11 %.)
-template <typename T, int D, bool kList>
+// kList: the items come from the list; else every CTA has at most one, which it finds itself.  kDual: Shape::dual.  (Template parameters: with a branch on the
+// first head_dim 64 lost 11 %.)
+template <typename T, int D, bool kList, bool kDual>
 __global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __grid_constant__ TmaMaps maps, PackedParams p, Shape shape, const Plan* plan, const Item* items) {
     using C = Cfg<D>;
     extern __shared__ unsigned char smem_dyn[];
@@ -327,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __gri
         dst[0] = src[0]; dst[1] = src[1];
         return w;
     };
-    auto head_of = [&](int idx) { return idx % shape.head_blocks * shape.fold; };      // first head of the block
+    auto head_of = [&](int idx) { return idx % shape.head_blocks * (kDual ? 2 * shape.fold : shape.fold); };      // first head of the item
 
     if (warp >= 8) {
         reg_dec<kRegOther>();
@@ -346,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __gri
                     mbar_arrive_expect_tx(&bar->q_full[b], C::kQTile);
 #pragma unroll
                     for (int h = 0; h < C::kHalves; ++h)
-                        tma_load_4d(q_smem + b * C::kQTile + h * C::kQHalf, &maps.q, &bar->q_full[b], h * 64, head, w.q0 + t * shape.tokens, 0);
+                        tma_load_4d(q_smem + b * C::kQTile + h * C::kQHalf, &maps.q, &bar->q_full[b], h * 64, kDual ? head + t * shape.fold : head, kDual ? w.q0 : w.q0 + t * shape.tokens, 0);
                 };
                 int round = 0, idx = -1;
                 while (round < n_rounds && (idx = item_of_round(round, n_items)) < 0) ++round;
@@ -362,17 +377,19 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __gri
                     if (idx2 >= 0) { wn = item_of(idx2); head2 = head_of(idx2); load_q(wn, head2, 0); }
                     const int nmax = blocks_of(max(w.end[0], w.end[1]), C::kN);
                     // in the order in which the products take them: K0, then K(j+1), V(j)
-                    for (int x = 0; x < 2 * nmax && ok; ++x, ++kv_item) {
-                        const int slot = kv_item % C::kStages;
-                        if (kv_item >= C::kStages) ok = mbar_wait(&bar->kv_empty[slot], ((kv_item / C::kStages) - 1) & 1, abort_flag, 0x100);
-                        if (!ok) break;
+                    for (int x = 0; x < 2 * nmax && ok; ++x) {
                         const bool value = x == 2 * nmax - 1 || (x > 0 && (x & 1) == 0);
                         const int block = x == 0 ? 0 : value ? (x - 1) / 2 : (x + 1) / 2;
-                        mbar_arrive_expect_tx(&bar->kv_full[slot], C::kKvTile);
                         const CUtensorMap* m = value ? &maps.v : &maps.k;
+                        for (int t = 0; t < (kDual ? 2 : 1); ++t, ++kv_item) {          // (dual: tile 0's block, then tile 1's)
+                            const int slot = kv_item % C::kStages;
+                            if (kv_item >= C::kStages) ok = mbar_wait(&bar->kv_empty[slot], ((kv_item / C::kStages) - 1) & 1, abort_flag, 0x100);
+                            if (!ok) break;
+                            mbar_arrive_expect_tx(&bar->kv_full[slot], C::kKvTile);
 #pragma unroll
-                        for (int h = 0; h < C::kHalves; ++h)
-                            tma_load_4d(kv_smem + slot * C::kKvTile + h * C::kKvHalf, m, &bar->kv_full[slot], h * 64, head / rep, w.k0 + block * C::kN, 0);
+                            for (int h = 0; h < C::kHalves; ++h)
+                                tma_load_4d(kv_smem + slot * C::kKvTile + h * C::kKvHalf, m, &bar->kv_full[slot], h * 64, (head + t * shape.fold) / rep, w.k0 + block * C::kN, 0);
+                        }
                     }
                     if (idx2 >= 0) load_q(wn, head2, 1);
                     idx = idx2; round = round2; w = wn; head = head2;
@@ -406,6 +423,13 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __gri
                 };
                 int slot = 0, kv_phase = 0, qb = 0, q_phase = 0;
                 auto next_slot = [&]() { if (++slot == C::kStages) { slot = 0; kv_phase ^= 1; } };
+                // a block of the other tile's: handed back when it has come, so that the slot's turns stay in step
+                auto skip = [&]() {
+                    if (!mbar_wait(&bar->kv_full[slot], kv_phase, abort_flag, 0x201)) return false;
+                    mbar_arrive(&bar->kv_empty[slot]);
+                    next_slot();
+                    return true;
+                };
                 uint32_t s_phase = 1, p_phase = 0;               // (the first wait for free scores passes: none have been made)
                 bool ok = true;
                 for (int round = 0; round < n_rounds && ok; ++round) {
@@ -425,7 +449,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __gri
                     // j = -1: the first scores; then the scores of block j + 1 and the weighted values of block j
                     for (int j = -1; j < nmax && ok; ++j) {
                         if (j + 1 < nmax) {
-                            ok = mbar_wait(&bar->kv_full[slot], kv_phase, abort_flag, 0x200);
+                            if (kDual && t == 1) ok = skip();
+                            ok = ok && mbar_wait(&bar->kv_full[slot], kv_phase, abort_flag, 0x200);
                             if (!ok) break;
                             if (j + 1 < n) {
                                 // the scores before these, of this item or the one before it, have been read
@@ -444,9 +469,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __gri
                                 mbar_arrive(&bar->kv_empty[slot]);                    // a block for the other tile
                             }
                             next_slot();
+                            if (kDual && t == 0) ok = skip();
                         }
                         if (j < 0) continue;
-                        ok = mbar_wait(&bar->kv_full[slot], kv_phase, abort_flag, 0x300);
+                        if (kDual && t == 1) ok = ok && skip();
+                        ok = ok && mbar_wait(&bar->kv_full[slot], kv_phase, abort_flag, 0x300);
                         if (!ok) break;
                         if (j < n) {
                             const int rows = w.keys - j * C::kN;        // of the sequence in this block of V
@@ -470,6 +497,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __gri
                             mbar_arrive(&bar->kv_empty[slot]);
                         }
                         next_slot();
+                        if (kDual && t == 0) ok = skip();
                     }
                 }
                 // everything issued so far has to retire before TMEM is released
@@ -483,7 +511,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __gri
         reg_inc<kRegSoftmax>();
         const int t = warp >> 2;                     // tile of this warpgroup
         const int r = tid & 127;                     // row inside the tile = TMEM lane
-        const int token = t * shape.tokens + r / shape.fold, head_in = r % shape.fold;
+        const int first = kDual ? 0 : t * shape.tokens;      // of the tile's tokens
+        const int token = first + r / shape.fold, head_in = r % shape.fold + (kDual ? t * shape.fold : 0);
         const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_addr = tmem_base + lane_base + (t ? C::kS(1) : C::kS(0));
         const uint32_t p_addr = tmem_base + lane_base + (t ? C::kP(1) : C::kP(0));
@@ -501,7 +530,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __gri
             if (tile_end < 0) continue;                                     // no tokens in this tile
             const int n = blocks_of(tile_end, C::kN);
             const int limit = p.causal ? min(w.keys - 1, w.last + token) : w.keys - 1;      // last visible key of this row
-            const int all_see = p.causal ? min(w.keys, w.last + t * shape.tokens + 1) : w.keys;      // keys that every row of the tile sees
+            const int all_see = p.causal ? min(w.keys, w.last + first + 1) : w.keys;      // keys that every row of the tile sees
 
             float m_ref = -INFINITY;
             float2 rs[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};      // partial sums of the weights
@@ -685,19 +714,19 @@ struct Carve {
 Carve carve(int batch, const Shape& s) {
     Carve c;
     c.items = 256;
-    c.first = c.items + up256(sizeof(Item) * static_cast<size_t>(s.max_items));
+    c.first = c.items + up256(sizeof(Item) * static_cast<size_t>(s.room));
     c.total = c.first + up256(sizeof(int) * (static_cast<size_t>(batch) + 1));
     return c;
 }
 
-template <typename T, int D, bool kList>
+template <typename T, int D, bool kList, bool kDual>
 int launch_t(cudaStream_t s, const PackedParams& p, const Shape& shape, int64_t most) {
     static thread_local bool configured[64] = {};      // per device ordinal: the attribute belongs to the device's context
     int dev = 0;
     VB200_CUDA_TRY(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64) return set_detail(VB200_ERR_NO_DEVICE, "device ordinal out of range");
     if (!configured[dev]) {
-        VB200_CUDA_TRY(cudaFuncSetAttribute(prefill_packed_kernel<T, D, kList>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmemBytes));
+        VB200_CUDA_TRY(cudaFuncSetAttribute(prefill_packed_kernel<T, D, kList, kDual>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmemBytes));
         configured[dev] = true;
     }
     const Carve c = carve(p.batch, shape);
@@ -712,7 +741,7 @@ int launch_t(cudaStream_t s, const PackedParams& p, const Shape& shape, int64_t 
     if (int rc = make_map(&maps.k, p.dtype, k, n_k, h_k, D, 1, Cfg<D>::kN)) return rc;
     if (int rc = make_map(&maps.v, p.dtype, v, n_k, h_k, D, 1, Cfg<D>::kN)) return rc;
     if (kList) {
-        packed_plan_kernel<<<1, kPlanThreads, 0, s>>>(p, shape.tokens, shape.max_items, plan, items, reinterpret_cast<int*>(ws + c.first));
+        packed_plan_kernel<<<1, kPlanThreads, 0, s>>>(p, shape, plan, items, reinterpret_cast<int*>(ws + c.first));
         note_launch();
         VB200_CUDA_TRY(cudaPeekAtLastError());
     }
@@ -727,7 +756,7 @@ int launch_t(cudaStream_t s, const PackedParams& p, const Shape& shape, int64_t 
     cfg.attrs = attr;
     cfg.numAttrs = kList ? 1 : 0;
     profile_mark_begin(s);
-    VB200_CUDA_TRY(cudaLaunchKernelEx(&cfg, prefill_packed_kernel<T, D, kList>, maps, p, shape, static_cast<const Plan*>(plan), static_cast<const Item*>(items)));
+    VB200_CUDA_TRY(cudaLaunchKernelEx(&cfg, prefill_packed_kernel<T, D, kList, kDual>, maps, p, shape, static_cast<const Plan*>(plan), static_cast<const Item*>(items)));
     profile_mark_end(s);
     note_launch();
     return VB200_OK;
@@ -738,13 +767,16 @@ int launch_t(cudaStream_t s, const PackedParams& p, const Shape& shape, int64_t 
 size_t prefill_packed_workspace(int batch, int Hq, int Hkv, int total_q) { return carve(batch, shape_of(batch, Hq, Hkv, total_q)).total; }
 
 int launch_prefill_packed(cudaStream_t s, const PackedParams& p) {
-    const Shape shape = shape_of(p.batch, p.Hq, p.Hkv, p.total_q);
+    Shape shape = shape_of(p.batch, p.Hq, p.Hkv, p.total_q);
+    if (two_head_blocks(p, shape)) shape = shape_of(p.batch, p.Hq, p.Hkv, p.total_q, true);
     const int64_t most = static_cast<int64_t>(shape.max_items) * shape.head_blocks;
     // With an item per SM at most, a CTA finds its own: no list, and one launch less (eight requests of 5-96 tokens, 16 heads on 4: 9.8 us, with the list 11.6).
     const bool list = most > device_sm_count();
     auto go = [&](auto t, auto d) {
         using T = decltype(t);
-        return list ? launch_t<T, decltype(d)::value, true>(s, p, shape, most) : launch_t<T, decltype(d)::value, false>(s, p, shape, most);
+        constexpr int D = decltype(d)::value;
+        if (shape.dual) return list ? launch_t<T, D, true, true>(s, p, shape, most) : launch_t<T, D, false, true>(s, p, shape, most);
+        return list ? launch_t<T, D, true, false>(s, p, shape, most) : launch_t<T, D, false, false>(s, p, shape, most);
     };
     using D64 = std::integral_constant<int, 64>;
     using D128 = std::integral_constant<int, 128>;
