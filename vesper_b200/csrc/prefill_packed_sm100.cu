@@ -13,11 +13,13 @@
 //   warp  8      TMA: q tiles (3 buffers, so that the next item's come while this one computes) and the ring of key and value blocks
 //   warps 9, 10  tcgen05.mma issuers of tile 0 and of tile 1; warp 9 owns the TMEM
 // TMEM (512 columns): per tile the scores S of a block, its weights (16 bits, two to a column) beside them, and O.  The weights do not overwrite the scores, so
-// that the next block's Q K^T is made while this block's weights are computed: with head_dim 128 a block is 80 keys (2 x (80 + 40 + 128) columns), with 64 it
-// is 128 keys (2 x (128 + 64 + 64)).  (Blocks of 128 keys whose weights overwrote their scores, head_dim 128: 518 us for 24 prompts of 16-4057 tokens, tensor
-// pipe busy 49 %, the softmax and the products of a tile waiting for each other.)
+// that the next block's Q K^T is made while this block's weights are computed: with head_dim 128 a block is 80 keys (2 x (80 + 40 + 128) columns), with 64 it is
+// 112 (2 x (112 + 56 + 64); 128 would fit, and its scores spill registers).  (Blocks of 128 keys whose weights overwrote their scores, head_dim 128: 518 us for 24
+// prompts of 16-4057 tokens, tensor pipe busy 49 %, the softmax and the products of a tile waiting for each other.)
 // The last block of a tile takes only the columns and rows of V, by 16, that a row of it can see.  The rows of V behind the sequence in its last
 // 16 are another sequence's, or nobody's: they are cleared in shared memory, since a weight of zero does not silence a NaN.
+// What bounds it: the softmax and the products of a tile in turn (long portions: tensor pipe 67 %, special function unit 59 %).  Causal, 32 heads on 8 of 128: 24
+// prompts of 16-4057 tokens 490 us, 1054 TFLOP/s; not causal: 8192 tokens 830 us, 1324 TFLOP/s, with 32 key heads of 64 710-745 us, 774 TFLOP/s.
 // Every wait is bounded (mbar_wait); on expiry the CTA drains and returns with the status word set.
 #include "hybrid.cuh"
 #include "serving.h"
@@ -209,7 +211,7 @@ template <int D>
 struct Cfg {
     static constexpr int kN = D == 128 ? 80 : 112;               // keys of a block
     static constexpr int kStages = D == 128 ? 6 : 8;             // key / value slots
-    static constexpr int kOnFma = 1;
+    static constexpr int kOnFma = 1;                             // of 8 pairs of weights: 1337 TFLOP/s at 8192 x 8192 keys, 0 gives 1280 and 2 1267
     static constexpr int kHalves = D / 64;                       // 64-column (128-byte) boxes per row
     static constexpr int kQHalf = kBlockM * 128, kQTile = kHalves * kQHalf;
     static constexpr int kKvHalf = kN * 128, kKvTile = kHalves * kKvHalf;

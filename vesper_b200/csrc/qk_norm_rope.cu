@@ -7,6 +7,7 @@
 // What bounds it: HBM, each element is read once and written once.  A row of D elements is held by D / 16 neighbouring threads, 16 elements each, which
 // sum the squares with shuffles.  A CTA takes a few tokens and a share of their heads: the angles of a token are computed once
 // per CTA, while its first rows are on their way, and read from shared memory by all of its heads; the rows of a packed projection lie next to each other.
+// 8191 tokens of 32 + 8 heads of 128, bf16: 34 us, 4.9 TB/s, issue slots 60 % busy with shuffles and reads of the angles; 65536 tokens 228 us, 5.9 TB/s.
 #include "hybrid.cuh"
 #include "serving.h"
 
