@@ -31,8 +31,7 @@ typedef struct vb200_rows {
  * by the angle position * inv_freq[i] (rope.enabled == 0: not turned); all in fp32, rounded once.  The product position * inv_freq[i] is not rounded
  * to fp32 as apply_rotary_emb does it (a thousandth of a radian at position 16384): rotate the queries and the keys of one cache with one of the two.
  * Outputs stand like the inputs (and may be the same memory: q_out == q with the same strides; overlapping otherwise is not allowed, and neither are negative
- * strides), or, with
- * dst.rows, k_out and v_out are [dst.seqs, Hkv, dst.cap, D] caches and token (b, t) is written where `dst` says.
+ * strides, and strides of 0 in an output where there is more than one), or, with dst.rows, k_out and v_out are [dst.seqs, Hkv, dst.cap, D] caches and token (b, t) is written where `dst` says.
  * Any of q, k, v may be left out (ptr null together with its output's); v is copied, which needs an output of its own. */
 typedef struct vb200_qk_norm_rope_args {
     size_t struct_size;

@@ -92,6 +92,26 @@ def test_norm_refuses_views(serving):
     assert call(dst=serving.Rows(None, P, 0, 0)) == -1 and call(dst=serving.Rows(P, None, 0, 8)) == -1 and call(dst=serving.Rows(P, None, 2, 0)) == -1
 
 
+def test_outputs_may_not_be_broadcast(serving):
+    """An element that several results would be written to (or, in place, that several would read): refused; a dimension of one may have any stride."""
+    from vesper_b200 import capi
+    L = serving.load()
+    norm = lambda **kw: L.vb200_qk_norm_rope(C.byref(norm_args(serving, **kw)))  # noqa: E731
+    H, T = 8 * 5 * 128, 5 * 128
+    for strides in ((0, T, 128), (H, 0, 128), (H, T, 0)):
+        assert norm(q_out=capi.Tensor4(P, *strides)) == -2 and norm(k_out=capi.Tensor4(P, *strides)) == -2 and norm(v_out=capi.Tensor4(P, *strides)) == -2
+        cache = serving.Rows(P, None, 4, 64)
+        assert norm(dst=cache, k_out=capi.Tensor4(P, *strides)) == -2
+        read = rows_args(serving, k=capi.Tensor4(P, *strides))
+        assert L.vb200_kv4_read(C.byref(read)) == -2
+        read = rows_args(serving, v=capi.Tensor4(P, *strides))
+        assert L.vb200_kv4_read(C.byref(read)) == -2
+    assert norm(dst=serving.Rows(P, None, 4, 64), T=1, k_out=capi.Tensor4(P, H, T, 0)) == -2                 # the cache has more rows than the call has tokens
+    assert norm(T=1, q_out=capi.Tensor4(P, H, T, 0), q=capi.Tensor4(P + 2, H, T, 0)) == -3                  # (not refused for its stride)
+    for strides in ((0, 128, 128), (1024, 0, 128)):
+        assert L.vb200_decode_kv4_fwd(C.byref(decode_args(serving, o=capi.Tensor4(P, *strides)))) == -2
+
+
 def packed_args(serving, **kw):
     from vesper_b200 import capi
     t = lambda H: capi.Tensor4(P, 0, 128, H * 128)  # noqa: E731
@@ -231,3 +251,7 @@ def test_wrapper_refuses(serving):
         serving._whole("rows", torch.zeros(8, dtype=torch.int64), torch.int32, -1, 8)
     c = serving.Kv4Cache(2, 3, 60, 128, device="cpu")
     assert c.cap == 64 and c.view.stride_h == 64 and c.view.stride_b == 192
+    with pytest.raises(ValueError):
+        serving._workspace(torch.zeros(64, 2, dtype=torch.uint8)[:, 0], 0, x(1), None)
+    with pytest.raises(ValueError):
+        serving._code(torch.zeros(1, dtype=torch.float64))

@@ -27,6 +27,10 @@ vb200_tensor4 used(vb200_tensor4 t, int64_t B, int64_t H, int64_t S) {
     return t;
 }
 
+// an output: no element stands for several (a dimension of extent 1 may have any stride)
+bool written_once(const vb200_tensor4& t, int64_t B, int64_t H, int64_t S) { return (B <= 1 || t.stride_b != 0) && (H <= 1 || t.stride_h != 0) && (S <= 1 || t.stride_s != 0); }
+int broadcast_output() { return set_detail(VB200_ERR_UNSUPPORTED, "outputs may not be broadcast: a stride of 0 where there is more than one"); }
+
 // f / (2 pi) as a fraction of 2^64, whole turns dropped: f = m * 2^e with a whole m of 24 bits, times 2^100 / (2 pi) as a whole number
 unsigned long long turn_fraction(float f) {
     int e = 0;
@@ -82,6 +86,7 @@ int check_kv4_rows(const vb200_kv4_rows_args* a, bool writing) {
         if (a->start_row < 0 || static_cast<int64_t>(a->start_row) + a->T > a->cache.cap) return set_detail(VB200_ERR_INVALID_ARG, "start_row + T exceeds the cache capacity");
         if (a->B > a->cache.seqs) return set_detail(VB200_ERR_INVALID_ARG, "B exceeds the cache's sequences");
     }
+    if (!writing && ((a->k.ptr && !written_once(a->k, a->B, a->Hkv, a->T)) || (a->v.ptr && !written_once(a->v, a->B, a->Hkv, a->T)))) return broadcast_output();
     if ((a->k.ptr && !view_aligned(used(a->k, a->B, a->Hkv, a->T), 2)) || (a->v.ptr && !view_aligned(used(a->v, a->B, a->Hkv, a->T), 2)))
         return set_detail(VB200_ERR_ALIGNMENT, "k / v base and strides must be 16-byte aligned");
     return VB200_OK;
@@ -185,6 +190,7 @@ int vb200_qk_norm_rope(const vb200_qk_norm_rope_args* a) {
     for (int i = 0; i < 3; ++i) {
         if (!in[i]->ptr) continue;
         const bool to_cache = scatter && i > 0;
+        if (to_cache ? !written_once(*out[i], a->dst.seqs, heads[i], a->dst.cap) : !written_once(*out[i], a->B, heads[i], a->T)) return broadcast_output();
         if (!view_aligned(used(*in[i], a->B, heads[i], a->T), size) ||
             !view_aligned(to_cache ? used(*out[i], a->dst.seqs, heads[i], a->dst.cap) : used(*out[i], a->B, heads[i], a->T), size))
             return set_detail(VB200_ERR_ALIGNMENT, "q / k / v and outputs: base and strides must be 16-byte aligned");
@@ -267,6 +273,7 @@ int vb200_decode_kv4_fwd(const vb200_decode_kv4_args* a) {
     const int64_t most = a->max_len > 0 ? std::min(a->max_len, a->cache.cap) : a->cache.cap;
     if (!a->seq_lens && (a->uniform_len < 0 || static_cast<int64_t>(a->uniform_len) + append > most)) return set_detail(VB200_ERR_INVALID_ARG, "uniform_len out of range for the cache or max_len");
     if (a->advance_lens && !a->seq_lens) return set_detail(VB200_ERR_INVALID_ARG, "advance_lens needs seq_lens");
+    if (!written_once(a->o, a->B, a->Hq, 1)) return broadcast_output();
     if (!view_aligned(used(a->q, a->B, a->Hq, 1), 2) || !view_aligned(used(a->o, a->B, a->Hq, 1), 2) ||
         (append && (!view_aligned(used(a->k_new, a->B, a->Hkv, 1), 2) || !view_aligned(used(a->v_new, a->B, a->Hkv, 1), 2))))
         return set_detail(VB200_ERR_ALIGNMENT, "q / k_new / v_new / o base and strides must be 16-byte aligned");

@@ -78,6 +78,8 @@ def _code(t):
     if not _TYPES:
         import torch
         _TYPES.update({torch.float32: capi.F32, torch.bfloat16: capi.BF16, torch.float16: capi.F16})
+    if t.dtype not in _TYPES:
+        raise ValueError(f"expected float32, bfloat16 or float16, got {t.dtype}")
     return _TYPES[t.dtype]
 
 
@@ -131,6 +133,8 @@ def _rows(rows, seqs, device, tokens, n_seqs, cap):
 def _workspace(workspace, need, t, stream):
     if workspace is None:
         workspace = capi._workspace(need, t.device, stream)
+    elif workspace.get_device() != t.get_device() or not workspace.is_contiguous():
+        raise ValueError(f"workspace: expected contiguous memory on {t.device}, got one on {workspace.device}, strides {workspace.stride()}")
     return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
@@ -173,7 +177,7 @@ def qk_norm_rope(q, k, v=None, *, eps=None, q_weight=None, k_weight=None, theta=
         if numpy is not None and numpy["typestr"] == "<f4" and numpy["strides"] is None:
             turned, table = 1, numpy["data"][0]
         else:
-            if not isinstance(inv_freq, C.Array):
+            if not (isinstance(inv_freq, C.Array) and inv_freq._type_ is C.c_float):
                 inv_freq = (C.c_float * (D // 2))(*[float(x) for x in inv_freq])
             turned, table = 1, C.addressof(inv_freq)
     a = _NORM.pack(_NORM.size, device, _stream(device, stream), _code(some), B, Hq, Hkv, T, D,
