@@ -5,12 +5,13 @@
 //
 // A tile is 128 rows: 128 / F tokens of one sequence by F heads of one key head's group (F: the power of two of the group, at most 16), row = token * F +
 // head, as one TMA box of q brings them.  Short sequences fill a tile with heads instead of padding, and the rows of a tile see nearly the same keys.  A work
-// item is two tiles of neighbouring tokens that read the same blocks of keys; where the sequences are
-// short, two blocks of heads of the same tokens (two_head_blocks).  The lengths are on the device: a first kernel lists the items with the longest first, then
-// persistent CTAs, one per SM, take them in snake order.
+// item is two tiles of neighbouring tokens that read the same blocks of keys; where the sequences are short, two blocks of heads of the same tokens
+// (two_head_blocks).  The lengths are on the device: a first kernel lists the items with the longest first, then persistent CTAs, one per SM, take the next one
+// of the list as they get done.  (Dealt out beforehand, up and down the CTAs: 492 us instead of 473 for 24 prompts of 16-4057 tokens, 32 heads on 8 of 128; 62
+// instead of 55 for 17 of 100-1500, 16 heads on 2.)
 //   warps 0-3    softmax and epilogue of tile 0, a row per thread (TMEM lane)
 //   warps 4-7    the same for tile 1
-//   warp  8      TMA: q tiles (3 buffers, so that the next item's come while this one computes) and the ring of key and value blocks
+//   warp  8      the items, which it tells the others of; TMA: q tiles (3 buffers, so that the next item's come while this one computes) and the ring of key and value blocks
 //   warps 9, 10  tcgen05.mma issuers of tile 0 and of tile 1; warp 9 owns the TMEM
 // TMEM (512 columns): per tile the scores S of a block, its weights (16 bits, two to a column) beside them, and O.  The weights do not overwrite the scores, so
 // that the next block's Q K^T is made while this block's weights are computed: with head_dim 128 a block is 80 keys (2 x (80 + 40 + 128) columns), with 64 it is
@@ -19,7 +20,7 @@
 // The last block of a tile takes only the columns and rows of V, by 16, that a row of it can see.  The rows of V behind the sequence in its last
 // 16 are another sequence's, or nobody's: they are cleared in shared memory, since a weight of zero does not silence a NaN.
 // What bounds it: the softmax and the products of a tile in turn (long portions: tensor pipe 67 %, special function unit 59 %).  Causal, 32 heads on 8 of 128: 24
-// prompts of 16-4057 tokens 490 us, 1054 TFLOP/s; not causal: 8192 tokens 830 us, 1324 TFLOP/s, with 32 key heads of 64 710-745 us, 774 TFLOP/s.
+// prompts of 16-4057 tokens 473 us, 1092 TFLOP/s; not causal: 8192 tokens 830 us, 1324 TFLOP/s, with 32 key heads of 64 725 us, 758 TFLOP/s.
 // Every wait is bounded (mbar_wait); on expiry the CTA drains and returns with the status word set.
 #include "hybrid.cuh"
 #include "serving.h"
@@ -46,11 +47,13 @@ static_assert(kRegSoftmax * 256 + kRegOther * 128 <= 168 * 384, "register budget
 // sees is `last` + i (causal).
 struct alignas(16) Item {
     int q0, tokens, k0, keys;
-    int last, end[2], pad;                 // keys that some row of each tile sees; -1: the tile has no tokens
+    int last, end[2];                      // keys that some row of each tile sees; -1: the tile has no tokens
+    int head;                              // first head of the block (set as the item is taken from the list)
 };
 
 struct Plan {                              // workspace: the header, the items, the first item of each sequence
     int items;
+    int next;                              // item that the next CTA in want of one takes
 };
 
 struct Shape {
@@ -106,7 +109,7 @@ __device__ __forceinline__ Item make_item(const PackedParams& p, const Shape& sh
     w.k0 = s.k0;
     w.keys = s.nk;
     w.last = p.causal ? s.nk - s.nq + r0 : s.nk - 1;
-    w.pad = 0;
+    w.head = 0;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         const int first = shape.dual ? 0 : t * shape.tokens;                 // of the tile's tokens
@@ -118,7 +121,7 @@ __device__ __forceinline__ Item make_item(const PackedParams& p, const Shape& sh
 
 constexpr int kAtHand = 1024;              // sequences that the planning block keeps in shared memory
 
-__global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedParams p, Shape shape, Plan* plan, Item* items, int* first_in_memory) {
+__global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedParams p, Shape shape, int ctas, Plan* plan, Item* items, int* first_in_memory) {
     __shared__ int hist[kBins];
     __shared__ long long warp_sum[32];
     __shared__ int first_at_hand[kAtHand + 1];
@@ -168,6 +171,7 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedParams 
         const int n = static_cast<int>(min(next, static_cast<long long>(max_items)));      // (offsets in order leave no more than max_items)
         first_item[p.batch] = n;
         plan->items = n;
+        plan->next = 2 * ctas;                           // (CTA c starts with the items c and 2 ctas - 1 - c)
     }
     __syncthreads();
     const int n = first_item[p.batch];
@@ -194,11 +198,14 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedParams 
 }
 
 // ---- the attention kernel ----
-struct __align__(8) Barriers {
+constexpr int kBoxes = 4;
+struct __align__(16) Barriers {
     uint64_t q_full[kQBufs], q_free[kQBufs];
     uint64_t kv_full[8], kv_empty[8];
     uint64_t s_full[2], s_free[2], p_ready[2], o_done[2];
     uint64_t mma_done;
+    uint64_t box_full[kBoxes], box_empty[kBoxes];
+    Item box[kBoxes];                      // the producer's word to the other warps; no tokens: no more items
     uint32_t tmem_base;
     int abort_flag;
 };
@@ -219,18 +226,10 @@ struct Cfg {
     static constexpr int kS(int t) { return t * (D == 128 ? 128 : kTile); }
     static constexpr int kP(int t) { return kS(t) + kN; }
     static constexpr int kO(int t) { return 512 - (2 - t) * D; }
-    static constexpr int kSmemBytes = kQBufs * kQTile + kStages * kKvTile + 1024 /*alignment slack*/ + 256 /*Barriers*/;
+    static constexpr int kSmemBytes = kQBufs * kQTile + kStages * kKvTile + 1024 /*alignment slack*/ + sizeof(Barriers);
     static_assert(kP(1) + kN / 2 <= kO(0) && kStages <= 8 && kSmemBytes <= 227 * 1024, "layout");
 };
 __device__ __forceinline__ int blocks_of(int end, int n) { return end > 0 ? (end + n - 1) / n : 0; }
-static_assert(sizeof(Barriers) <= 256, "room for the barriers");
-
-// Round r gives CTA c item r * G + c (even r) or r * G + G - 1 - c (odd r), which evens out the sums.  -1: none.
-__device__ __forceinline__ int item_of_round(int round, int n_items) {
-    const int G = gridDim.x, c = blockIdx.x;
-    const int idx = round * G + ((round & 1) ? (G - 1 - c) : c);
-    return idx < n_items ? idx : -1;
-}
 
 template <int N> __device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -292,7 +291,7 @@ __device__ __forceinline__ bool find_item(const PackedParams& p, const Shape& sh
 // kList: the items come from the list; else every CTA has at most one, which it finds itself.  kDual: Shape::dual.  (Template parameters: with a branch on the
 // first head_dim 64 lost 11 %.)
 template <typename T, int D, bool kList, bool kDual>
-__global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __grid_constant__ TmaMaps maps, PackedParams p, Shape shape, const Plan* plan, const Item* items) {
+__global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __grid_constant__ TmaMaps maps, PackedParams p, Shape shape, Plan* plan, const Item* items) {
     using C = Cfg<D>;
     extern __shared__ unsigned char smem_dyn[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));      // 128B-swizzled tiles
@@ -309,6 +308,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __gri
             for (int t = 0; t < 2; ++t) { mbar_init(&bar->s_full[t], 1); mbar_init(&bar->s_free[t], 4); mbar_init(&bar->p_ready[t], 4); mbar_init(&bar->o_done[t], 1); }
             for (int s = 0; s < C::kStages; ++s) { mbar_init(&bar->kv_full[s], 1); mbar_init(&bar->kv_empty[s], 2); }
             mbar_init(&bar->mma_done, 2);
+            for (int s = 0; s < kBoxes; ++s) { mbar_init(&bar->box_full[s], 1); mbar_init(&bar->box_empty[s], 10); }      // two issuers, eight warps
             bar->abort_flag = 0;
             mbar_fence_init();
         }
@@ -323,28 +323,36 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __gri
     tc_fence_after();
     asm volatile("griddepcontrol.wait;" ::: "memory");              // the list of items
     __shared__ Item own;
-    __shared__ int n_own;
+    const int head_step = kDual ? 2 * shape.fold : shape.fold;
     if constexpr (!kList) {
         if (warp == 0) {
             const bool found = find_item(p, shape, &own);
-            if (lane == 0) n_own = found ? gridDim.x : 0;
+            __syncwarp();
+            if (lane == 0) {
+                if (!found) own = Item{};
+                own.head = blockIdx.x % shape.head_blocks * head_step;
+            }
         }
         __syncthreads();
     }
     const uint32_t tmem_base = bar->tmem_base;
     const WaitCtx abort_flag{&bar->abort_flag, p.status};
-    const int n_items = kList ? plan->items * shape.head_blocks : n_own;
-    const int n_rounds = (n_items + gridDim.x - 1) / gridDim.x;
     const int rep = p.Hq / p.Hkv;
-    auto item_of = [&](int idx) {
-        Item w;
-        if constexpr (!kList) return own;
-        const int4* src = reinterpret_cast<const int4*>(items + idx / shape.head_blocks);
-        int4* dst = reinterpret_cast<int4*>(&w);
-        dst[0] = src[0]; dst[1] = src[1];
-        return w;
+    // the items of this CTA, one after the other, as the producer tells of them; null: no more (or a wait has expired)
+    int taken_items = 0;
+    auto take = [&](auto wait) -> const Item* {
+        const int n = taken_items++;
+        const Item* w = &own;
+        if constexpr (kList) {
+            const int s = n % kBoxes;
+            if (!wait(&bar->box_full[s], (n / kBoxes) & 1)) return nullptr;
+            w = &bar->box[s];
+        } else if (n > 0) {
+            return nullptr;
+        }
+        return w->tokens > 0 ? w : nullptr;
     };
-    auto head_of = [&](int idx) { return idx % shape.head_blocks * (kDual ? 2 * shape.fold : shape.fold); };      // first head of the item
+    auto give_back = [&]() { if (kList) mbar_arrive(&bar->box_empty[(taken_items - 1) % kBoxes]); };
 
     if (warp >= 8) {
         reg_dec<kRegOther>();
@@ -354,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __gri
                 int kv_item = 0;                 // running index into the ring over all items
                 int q_seq = 0;                   // running index of q tiles -> buffer q_seq % kQBufs
                 bool ok = true;
-                auto load_q = [&](const Item& w, int head, int t) {
+                auto load_q = [&](const Item& w, int t) {
                     if (w.end[t] <= 0 || !ok) return;
                     const int b = q_seq % kQBufs, use = q_seq / kQBufs;
                     if (use > 0) ok = mbar_wait(&bar->q_free[b], (use - 1) & 1, abort_flag, 0x110 + b);      // its last product has been made
@@ -363,20 +371,49 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __gri
                     mbar_arrive_expect_tx(&bar->q_full[b], C::kQTile);
 #pragma unroll
                     for (int h = 0; h < C::kHalves; ++h)
-                        tma_load_4d(q_smem + b * C::kQTile + h * C::kQHalf, &maps.q, &bar->q_full[b], h * 64, kDual ? head + t * shape.fold : head, kDual ? w.q0 : w.q0 + t * shape.tokens, 0);
+                        tma_load_4d(q_smem + b * C::kQTile + h * C::kQHalf, &maps.q, &bar->q_full[b], h * 64, kDual ? w.head + t * shape.fold : w.head, kDual ? w.q0 : w.q0 + t * shape.tokens, 0);
                 };
-                int round = 0, idx = -1;
-                while (round < n_rounds && (idx = item_of_round(round, n_items)) < 0) ++round;
-                Item w;
-                int head = 0;
-                if (idx >= 0) { w = item_of(idx); head = head_of(idx); load_q(w, head, 0); load_q(w, head, 1); }
-                while (idx >= 0 && ok) {
+                int told = 0;
+                auto tell = [&](const Item& w) {
+                    if constexpr (kList) {
+                        const int s = told % kBoxes;
+                        if (told >= kBoxes) ok = ok && mbar_wait(&bar->box_empty[s], (told / kBoxes - 1) & 1, abort_flag, 0x120);
+                        if (!ok) return;
+                        bar->box[s] = w;
+                        mbar_arrive(&bar->box_full[s]);
+                        ++told;
+                    }
+                };
+                auto item_of = [&](int idx) {
+                    Item w;
+                    const int4* src = reinterpret_cast<const int4*>(items + idx / shape.head_blocks);
+                    int4* dst = reinterpret_cast<int4*>(&w);
+                    dst[0] = src[0]; dst[1] = src[1];
+                    w.head = idx % shape.head_blocks * head_step;
+                    return w;
+                };
+                const int n_items = kList ? plan->items * shape.head_blocks : 0;
+                int next = 2 * gridDim.x - 1 - blockIdx.x;
+                Item w{};
+                if constexpr (!kList) w = own;
+                else if (static_cast<int>(blockIdx.x) < n_items) w = item_of(blockIdx.x);
+                load_q(w, 0);
+                tell(w);
+                load_q(w, 1);
+                while (w.tokens > 0 && ok) {
                     // one item ahead: its first q tile comes during this item
-                    int round2 = round + 1, idx2 = -1;
-                    while (round2 < n_rounds && (idx2 = item_of_round(round2, n_items)) < 0) ++round2;
-                    Item wn;
-                    int head2 = 0;
-                    if (idx2 >= 0) { wn = item_of(idx2); head2 = head_of(idx2); load_q(wn, head2, 0); }
+                    Item wn{};
+                    if (kList && next < n_items) {
+                        wn = item_of(next);
+                        next = atomicAdd(&plan->next, 1);                    // (looked at an item later)
+                    }
+                    bool announced = false;
+                    auto announce = [&]() {
+                        if (announced) return;
+                        announced = true;
+                        tell(wn);
+                        load_q(wn, 0);
+                    };
                     const int nmax = blocks_of(max(w.end[0], w.end[1]), C::kN);
                     // in the order in which the products take them: K0, then K(j+1), V(j)
                     for (int x = 0; x < 2 * nmax && ok; ++x) {
@@ -390,11 +427,13 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __gri
                             mbar_arrive_expect_tx(&bar->kv_full[slot], C::kKvTile);
 #pragma unroll
                             for (int h = 0; h < C::kHalves; ++h)
-                                tma_load_4d(kv_smem + slot * C::kKvTile + h * C::kKvHalf, m, &bar->kv_full[slot], h * 64, (head + t * shape.fold) / rep, w.k0 + block * C::kN, 0);
+                                tma_load_4d(kv_smem + slot * C::kKvTile + h * C::kKvHalf, m, &bar->kv_full[slot], h * 64, (w.head + t * shape.fold) / rep, w.k0 + block * C::kN, 0);
                         }
+                        if (x == 0) announce();                              // (the item has had this long to come)
                     }
-                    if (idx2 >= 0) load_q(wn, head2, 1);
-                    idx = idx2; round = round2; w = wn; head = head2;
+                    announce();
+                    load_q(wn, 1);
+                    w = wn;
                 }
             }
         } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
@@ -434,10 +473,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __gri
                 };
                 uint32_t s_phase = 1, p_phase = 0;               // (the first wait for free scores passes: none have been made)
                 bool ok = true;
-                for (int round = 0; round < n_rounds && ok; ++round) {
-                    const int idx = item_of_round(round, n_items);
-                    if (idx < 0) continue;
-                    const Item w = item_of(idx);
+                auto wait_item = [&](uint64_t* b, uint32_t parity) { return mbar_wait(b, parity, abort_flag, 0x230 + t); };
+                for (const Item* at; ok && (at = take(wait_item)) != nullptr;) {
+                    const Item w = *at;
+                    give_back();
                     const int end = t ? w.end[1] : w.end[0], n = blocks_of(end, C::kN), nmax = blocks_of(max(w.end[0], w.end[1]), C::kN);
                     // the q tiles of an item: tile 0's buffer, if it has one, then tile 1's
                     const bool q0 = w.end[0] > 0, q1 = w.end[1] > 0;
@@ -524,15 +563,17 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __gri
         int g = 0;                                   // running count of score tiles of this query tile
         bool ok = true;
 
-        for (int round = 0; round < n_rounds && ok; ++round) {
-            const int idx = item_of_round(round, n_items);
-            if (idx < 0) continue;
-            const Item w = item_of(idx);
-            const int tile_end = t ? w.end[1] : w.end[0];                   // keys that some row of the tile sees
+        auto wait_item = [&](uint64_t* b, uint32_t parity) { return mbar_wait_warp(b, parity, abort_flag, 0x810 + t); };
+        auto done = [&]() {                          // with the item: it stays in its box meanwhile, which leaves its registers to the scores
+            __syncwarp();
+            if (lane == 0) give_back();
+        };
+        for (const Item* w; ok && (w = take(wait_item)) != nullptr; done()) {
+            const int tile_end = t ? w->end[1] : w->end[0];                 // keys that some row of the tile sees
             if (tile_end < 0) continue;                                     // no tokens in this tile
             const int n = blocks_of(tile_end, C::kN);
-            const int limit = p.causal ? min(w.keys - 1, w.last + token) : w.keys - 1;      // last visible key of this row
-            const int all_see = p.causal ? min(w.keys, w.last + first + 1) : w.keys;      // keys that every row of the tile sees
+            const int limit = p.causal ? min(w->keys - 1, w->last + token) : w->keys - 1;      // last visible key of this row
+            const int all_see = p.causal ? min(w->keys, w->last + first + 1) : w->keys;      // keys that every row of the tile sees
 
             float m_ref = -INFINITY;
             float2 rs[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};      // partial sums of the weights
@@ -631,10 +672,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __gri
                 tc_fence_after();
             }
             const float l_sum = ((rs[0].x + rs[0].y) + (rs[1].x + rs[1].y)) + ((rs[2].x + rs[2].y) + (rs[3].x + rs[3].y));
-            const bool row_live = token < w.tokens;
+            const bool row_live = token < w->tokens;
             const float inv_l = l_sum == 0.f ? 0.f : 1.0f / l_sum;          // (a row that sees no key)
-            const int hq = head_of(idx) + head_in;
-            T* orow = static_cast<T*>(p.o.ptr) + hq * p.o.sh + static_cast<long long>(w.q0 + token) * p.o.ss;
+            const int hq = w->head + head_in;
+            T* orow = static_cast<T*>(p.o.ptr) + hq * p.o.sh + static_cast<long long>(w->q0 + token) * p.o.ss;
             const bool o32 = (reinterpret_cast<uintptr_t>(orow) & 31) == 0;     // every segment offset below is a multiple of 32 bytes
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
@@ -663,7 +704,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __gri
             // O has been read out: the next item's first PV (issued only after this thread's next p_ready arrival) may overwrite it
             tc_fence_before();
             if (p.lse != nullptr && row_live)
-                p.lse[static_cast<long long>(hq) * p.total_q + w.q0 + token] = l_sum == 0.f ? -INFINITY : (m_ref - kLift + fast_log2(l_sum)) * kLn2;
+                p.lse[static_cast<long long>(hq) * p.total_q + w->q0 + token] = l_sum == 0.f ? -INFINITY : (m_ref - kLift + fast_log2(l_sum)) * kLn2;
         }
     }
 
@@ -743,7 +784,7 @@ int launch_t(cudaStream_t s, const PackedParams& p, const Shape& shape, int64_t 
     if (int rc = make_map(&maps.k, p.dtype, k, n_k, h_k, D, 1, Cfg<D>::kN)) return rc;
     if (int rc = make_map(&maps.v, p.dtype, v, n_k, h_k, D, 1, Cfg<D>::kN)) return rc;
     if (kList) {
-        packed_plan_kernel<<<1, kPlanThreads, 0, s>>>(p, shape, plan, items, reinterpret_cast<int*>(ws + c.first));
+        packed_plan_kernel<<<1, kPlanThreads, 0, s>>>(p, shape, device_sm_count(), plan, items, reinterpret_cast<int*>(ws + c.first));
         note_launch();
         VB200_CUDA_TRY(cudaPeekAtLastError());
     }
@@ -758,7 +799,7 @@ int launch_t(cudaStream_t s, const PackedParams& p, const Shape& shape, int64_t 
     cfg.attrs = attr;
     cfg.numAttrs = kList ? 1 : 0;
     profile_mark_begin(s);
-    VB200_CUDA_TRY(cudaLaunchKernelEx(&cfg, prefill_packed_kernel<T, D, kList, kDual>, maps, p, shape, static_cast<const Plan*>(plan), static_cast<const Item*>(items)));
+    VB200_CUDA_TRY(cudaLaunchKernelEx(&cfg, prefill_packed_kernel<T, D, kList, kDual>, maps, p, shape, plan, static_cast<const Item*>(items)));
     profile_mark_end(s);
     note_launch();
     return VB200_OK;
