@@ -23,6 +23,7 @@ __global__ void __launch_bounds__(kThreads, kMinCtas) kv4_rows_kernel(Kv4RowsPar
     __shared__ long long at[kMaxTokens], row_of[kMaxTokens];                 // of a token, without the head: elements of k or v, and row of the cache (-1: left out)
     const bool value = blockIdx.y != 0;
     const View4& view = value ? p.v : p.k;
+    pdl_begin();
     if (!view.ptr) return;
     const int i0 = blockIdx.x * tokens_per_cta, n_tok = min(tokens_per_cta, p.B * p.T - i0);
     if (threadIdx.x < n_tok) {
@@ -108,10 +109,7 @@ template <typename T, int D, bool WRITE>
 int launch_t(cudaStream_t s, const Kv4RowsParams& p) {
     const long long total = static_cast<long long>(p.B) * p.T, fit = kMinCtas / 2 * static_cast<long long>(device_sm_count());
     const int tokens = static_cast<int>(std::min<long long>(kMaxTokens, (total + fit - 1) / fit));
-    kv4_rows_kernel<T, D, WRITE><<<dim3(static_cast<unsigned>((total + tokens - 1) / tokens), 2), kThreads, 0, s>>>(p, tokens);
-    note_launch();
-    VB200_CUDA_TRY(cudaPeekAtLastError());
-    return VB200_OK;
+    return launch_pdl(kv4_rows_kernel<T, D, WRITE>, dim3(static_cast<unsigned>((total + tokens - 1) / tokens), 2), dim3(kThreads), 0, s, p, tokens);
 }
 template <bool WRITE>
 int launch(cudaStream_t s, const Kv4RowsParams& p) {

@@ -183,6 +183,7 @@ template <typename T, int LANES>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 2) qk_norm_rope_kernel(QkNormRopeParams p, int tokens_per_cta, int heads_per_cta, int heads) {
     __shared__ Tokens tk;
     const int half = p.D / 2;
+    pdl_begin();
     const int total = p.B * p.T;
     const int i0 = blockIdx.x * tokens_per_cta, n_tok = min(tokens_per_cta, total - i0);
     const int h0 = blockIdx.y * heads_per_cta, h1 = min(h0 + heads_per_cta, heads);
@@ -229,10 +230,7 @@ int launch_t(cudaStream_t s, const QkNormRopeParams& p) {
     if (shares > heads) shares = heads;
     const int per = static_cast<int>((heads + shares - 1) / shares);
     const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>((heads + per - 1) / per));
-    qk_norm_rope_kernel<T, LANES><<<grid, kThreads, 0, s>>>(p, tokens, per, heads);
-    note_launch();
-    VB200_CUDA_TRY(cudaPeekAtLastError());
-    return VB200_OK;
+    return launch_pdl(qk_norm_rope_kernel<T, LANES>, grid, dim3(kThreads), 0, s, p, tokens, per, heads);
 }
 
 template <typename T>
