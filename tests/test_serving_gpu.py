@@ -264,6 +264,32 @@ def test_packed_workspace_of_the_largest_call(S):
         check_packed(q, k, v, o, lse, [each] * n, [each] * n, 0.125, True)
 
 
+def test_packed_two_calls_at_once(S):
+    """Two streams, a workspace each, and a graph replayed: the CTAs' counter of one call is not another's."""
+    lens = [300, 7, 0, 900, 64, 513] * 5
+    g = rng(21)
+    (q, k, v), cu, _ = packed_case(g, lens, lens, 16, 4, 128, torch.bfloat16)
+    o, lse = torch.empty_like(q), torch.empty(16, q.shape[0], device=DEV)
+    S.prefill_packed(q, k, v, o, lse, scale=0.09, cu_seqlens_q=cu)
+    check_packed(q, k, v, o, lse, lens, lens, 0.09, True)
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], [torch.zeros_like(q) for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for s, x in zip(streams, outs):
+            S.prefill_packed(q, k, v, x, scale=0.09, cu_seqlens_q=cu, stream=s)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], o) and torch.equal(outs[1], o)
+    x, workspace, graph = torch.zeros_like(q), S.prefill_packed_workspace(q, k, batch=len(lens)), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        S.prefill_packed(q, k, v, x, scale=0.09, cu_seqlens_q=cu, workspace=workspace)
+        S.prefill_packed(q, k, v, x, scale=0.09, cu_seqlens_q=cu, workspace=workspace)
+    for _ in range(2):
+        x.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(x, o)
+
+
 def test_packed_no_keys_at_all(S):
     g = rng(1)
     q = randn(g, 5, 4, 64)

@@ -121,7 +121,7 @@ __device__ __forceinline__ Item make_item(const PackedParams& p, const Shape& sh
 
 constexpr int kAtHand = 1024;              // sequences that the planning block keeps in shared memory
 
-__global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedParams p, Shape shape, int ctas, Plan* plan, Item* items, int* first_in_memory) {
+__global__ void __launch_bounds__(kPlanThreads, 1) packed_plan_kernel(PackedParams p, Shape shape, int ctas, Plan* plan, Item* items, int* first_in_memory) {
     __shared__ int hist[kBins];
     __shared__ long long warp_sum[32];
     __shared__ int first_at_hand[kAtHand + 1];
