@@ -57,9 +57,10 @@ int vb200_qk_norm_rope(const vb200_qk_norm_rope_args* a);
  * `batch` sequences stand one behind the other: the queries of sequence i are the tokens [cu_seqlens_q[i], cu_seqlens_q[i+1]) of q and o, its keys and
  * values the tokens [cu_seqlens_k[i], cu_seqlens_k[i+1]) of k and v (null: the same as cu_seqlens_q).  The lengths stay on the device.  Causal aligns
  * the last query with the last key: query i of n_q sees key j of n_k iff j <= n_k - n_q + i.  A query that sees no key gets zeros and an lse of
- * -infinity.  Tokens behind the last sequence are neither read (k, v) nor written (o, lse).  The running sums are fp32; the weights are rounded to
- * `dtype` for their product with v.  A non-finite value reaches every query of its sequence that sees a key of its block of at most 112 keys (a weight of zero
- * times infinity is NaN), as in vb200_prefill_fwd; it never reaches another sequence.
+ * -infinity; one whose scores are all -infinity gets NaN and an lse of -infinity (0 / 0 and ln 0).  Tokens behind the last sequence are neither read
+ * (k, v) nor written (o, lse).  The running sums are fp32; the weights are rounded to `dtype` for their product with v.  NaN in a key makes the results of the
+ * queries that see it NaN, the lse too.  A non-finite element of v reaches every query of its sequence that sees a key of its block of at most 112 keys (a
+ * weight of zero times infinity is NaN), as in vb200_prefill_fwd.  Neither ever reaches another sequence.
  * The offsets have to ascend and to stay within the tokens given.  A sequence whose own two do not is left out; nothing outside the tensors is read or
  * written whatever they are. */
 typedef struct vb200_prefill_packed_args {
