@@ -1,4 +1,4 @@
-"""Packed attention on values that are not finite: the columns of a tile of scores do not all take the same path."""
+"""Packed attention on values that are not finite, where the columns of a tile of scores do not all take the same path; 4-bit decode on queries of nothing."""
 import math
 
 import numpy as np
@@ -81,3 +81,26 @@ def test_every_score_minus_infinity(S, D, dtype, nk):
         o, lse = packed(S, q, k, v, 3, 1, 1, True)
         assert not o[0, :2].any() and bool((lse[:, 0, :2] == -math.inf).all())
         assert bool(torch.isnan(o[0, 2, :2]).all()) and bool((lse[:2, 0, 2] == -math.inf).all()) and torch.equal(o[0, 2, 2:], clean[0, 2, 2:])
+
+
+@pytest.mark.parametrize("size", [0.0, 2.0 ** -100])
+@pytest.mark.parametrize("exponent, scale", [(-64, 0.1), (-30, 0.1), (-25, 128 ** -0.5), (0, 1e-30), (64, 1e-38)])
+@pytest.mark.parametrize("Hq, Hkv, D", [(8, 2, 128), (2, 2, 64), (16, 1, 64)])
+def test_decode_kv4_queries_of_nothing(S, Hq, Hkv, D, exponent, scale, size):
+    """Queries of zero (a padded row of the batch), or nearly: the mean of the values and ln n, whatever the scale and the cache's exponents."""
+    lens = [1, 50, 64, 90, 300, 1000]
+    g = torch.Generator(device=DEV).manual_seed(D + exponent)
+    B, cap = len(lens), 1000
+    k, v = randn(g, B, Hkv, cap, D, scale=2.0 ** exponent), randn(g, B, Hkv, cap, D)
+    cache = S.Kv4Cache(B, Hkv, cap, D, device=DEV, k_exponent=exponent)
+    cache.append(k, v)
+    q = randn(g, B, Hq, 1, D, scale=size)
+    held_k, held_v = R.quantise(k, exponent), R.quantise(v)
+    for splits in (0, 1, 3):
+        o, lse = torch.full_like(q, 9.0), torch.full((B, Hq), 9.0, device=DEV)
+        S.decode_kv4(q, o, cache, scale=scale, lse=lse, seq_lens=int32(lens), num_splits=splits)
+        for b, n in enumerate(lens):
+            vv = held_v[b, :, :n].transpose(0, 1)
+            want, want_lse, weighted, score = R.attention(q[b].transpose(0, 1), held_k[b, :, :n].transpose(0, 1), vv, scale=scale, causal=False)
+            R.check(o[b].transpose(0, 1), want, R.attention_bound(want, weighted, score, dtype=q.dtype, weights=torch.float16, D=D, v=vv), f"o of {n} rows")
+            R.check(lse[b][:, None], want_lse, R.lse_bound(want_lse, score, D), f"lse of {n} rows")

@@ -270,7 +270,8 @@ __global__ void __launch_bounds__(kThreads, kMinCtas) decode_kv4_kernel(DecodeKv
             const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23), up = __uint_as_float(static_cast<uint32_t>(e) << 23);
             // the scale's sign goes into the queries, so that the largest product is the largest score
             const float sign = p.scale > 0.f ? 1.f : p.scale < 0.f ? -1.f : p.scale;
-            q_factor = sign == 0.f ? 1.f : fabsf(p.scale) * kLog2e * 8.0f * p.cache.k_unit * up;
+            // (never 0, which would make NaN of the -infinity of a masked score; below the least normal number, scores are nothing beside 1 whatever it is)
+            q_factor = sign == 0.f ? 1.f : fmaxf(fabsf(p.scale) * kLog2e * 8.0f * p.cache.k_unit * up, 1.17549435e-38f);
 #pragma unroll
             for (int w = 0; w < L::kKeyWords; ++w)
 #pragma unroll
