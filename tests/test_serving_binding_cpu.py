@@ -1,0 +1,76 @@
+"""The Python binding of the serving operators without a GPU: what it allocates, where and for how long, and what it refuses.  Tensors of the CPU say that they
+are on device 0, and the library's entry points are functions that look at what they are given."""
+import weakref
+
+import pytest
+import torch
+
+
+class OnDevice(torch.Tensor):
+    """A CPU tensor that calls itself one of device 0."""
+
+    def get_device(self):
+        return 0
+
+
+def zeros(*shape, dtype=torch.bfloat16):
+    return torch.zeros(*shape, dtype=dtype).as_subclass(OnDevice)
+
+
+class Library:
+    """Answers every entry point: sizes are 512 bytes, calls go to `seen` and succeed."""
+
+    def __init__(self):
+        self.seen, self.during = [], lambda: None
+
+    def __getattr__(self, name):
+        def entry(args):
+            if "_bytes" in name:
+                return 512
+            self.seen.append(name)
+            self.during()
+            return 0
+        return entry
+
+
+@pytest.fixture
+def serving(monkeypatch):
+    from vesper_b200 import serving_capi
+    library = Library()
+    monkeypatch.setattr(serving_capi, "load", lambda: library)
+    monkeypatch.setattr(serving_capi, "_stream", lambda device, stream: 0)
+    serving_capi.library = library
+    yield serving_capi
+    del serving_capi.library
+
+
+def packed_call(serving, **kw):
+    q, k = zeros(6, 4, 64), zeros(6, 2, 64)
+    return serving.prefill_packed(q, k, k, scale=0.1, cu_seqlens_q=zeros(3, dtype=torch.int32), **kw)
+
+
+def a_cache(serving):
+    u = lambda n: zeros(2, 2, 16, n, dtype=torch.uint8)  # noqa: E731
+    return serving.Kv4Cache(k_codes=u(32), v_codes=u(32), k_scales=u(2), v_scales=u(2))
+
+
+def decode_call(serving, **kw):
+    q = zeros(2, 4, 1, 64)
+    return serving.decode_kv4(q, torch.empty_like(q), a_cache(serving), scale=0.1, uniform_len=3, **kw)
+
+
+@pytest.mark.parametrize("call", [packed_call, decode_call])
+def test_the_workspace_lives_through_the_call(serving, monkeypatch, call):
+    """The one that the binding allocates is not another thread's, and not unmapped, before the kernels are launched; and it is let go of afterwards."""
+    made, alive = [], []
+    allocate = serving.capi._workspace
+
+    def workspace(*args, **kw):
+        t = allocate(*args, **kw)
+        made.append(weakref.ref(t))
+        return t
+    monkeypatch.setattr(serving.capi, "_workspace", workspace)
+    serving.library.during = lambda: alive.append([r() is not None for r in made])
+    call(serving)
+    assert alive == [[True]]
+    assert made[0]() is None

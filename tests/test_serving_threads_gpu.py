@@ -1,0 +1,72 @@
+"""The serving operators called from several host threads and streams at once."""
+import threading
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+
+
+@pytest.fixture(scope="module")
+def S(lib):
+    from vesper_b200 import serving_capi
+    return serving_capi
+
+
+def randn(g, *shape, dtype=torch.bfloat16):
+    return torch.randn(shape, generator=g, device=DEV).to(dtype)
+
+
+def int32(x):
+    return torch.tensor(np.asarray(x, dtype=np.int32), device=DEV)
+
+
+def together(works):
+    """Runs each in a thread of its own; raises what any of them raised."""
+    wrong = []
+
+    def run(work):
+        try:
+            torch.cuda.set_device(DEV)
+            work()
+        except BaseException as e:                                       # noqa: BLE001
+            wrong.append(e)
+    threads = [threading.Thread(target=run, args=(w,)) for w in works]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    if wrong:
+        raise wrong[0]
+
+
+def test_threads_on_one_stream_without_workspaces(S):
+    """Two threads share the default stream: each call's plan is read by its own attention kernel."""
+    batches = [[300, 7, 0, 900, 64, 513] * 3, [20, 40, 1500, 3] * 5, [2000]]
+    works, outs = [], []
+    for i, lens in enumerate(batches):
+        g = torch.Generator(device=DEV).manual_seed(i)
+        q, k, v = randn(g, sum(lens), 16, 128), randn(g, sum(lens), 4, 128), randn(g, sum(lens), 4, 128)
+        cu = int32(np.cumsum([0] + lens))
+        cache = S.Kv4Cache(len(lens), 4, 2008, 128, device=DEV)
+        k4 = randn(g, len(lens), 4, 2000, 128)
+        cache.append(k4, k4)
+        qd, seq = randn(g, len(lens), 16, 1, 128), int32(lens)
+        want, want_d = S.prefill_packed(q, k, v, scale=0.09, cu_seqlens_q=cu), S.decode_kv4(qd, torch.empty_like(qd), cache, scale=0.09, seq_lens=seq)
+        got = [(torch.zeros_like(q), torch.zeros_like(qd)) for _ in range(20)]
+        outs.append((want, want_d, got))
+
+        def work(q=q, k=k, v=v, cu=cu, cache=cache, qd=qd, seq=seq, got=got):
+            for o, od in got:
+                S.prefill_packed(q, k, v, o, scale=0.09, cu_seqlens_q=cu)
+                S.decode_kv4(qd, od, cache, scale=0.09, seq_lens=seq)
+        works.append(work)
+    torch.cuda.synchronize()
+    together(works)
+    torch.cuda.synchronize()
+    for want, want_d, got in outs:
+        for o, od in got:
+            assert torch.equal(o, want) and torch.equal(od, want_d)

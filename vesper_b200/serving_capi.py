@@ -131,11 +131,13 @@ def _rows(rows, seqs, device, tokens, n_seqs, cap):
 
 
 def _workspace(workspace, need, t, stream):
+    """(memory, address, bytes) of the caller's workspace or of a new one.  The caller holds on to the memory until its call has launched: before that, another
+    thread on the same stream could be given the same."""
     if workspace is None:
         workspace = capi._workspace(need, t.device, stream)
     elif workspace.get_device() != t.get_device() or not workspace.is_contiguous():
         raise ValueError(f"workspace: expected contiguous memory on {t.device}, got one on {workspace.device}, strides {workspace.stride()}")
-    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
 def qk_norm_rope(q, k, v=None, *, eps=None, q_weight=None, k_weight=None, theta=None, inv_freq=None, start_pos=0, positions=None, q_out=None, k_out=None, v_out=None,
@@ -213,7 +215,7 @@ def prefill_packed(q, k, v, o=None, lse=None, *, scale, cu_seqlens_q, cu_seqlens
     if cu_seqlens_k is None and tk < tq:
         raise ValueError("prefill_packed: fewer keys than queries need cu_seqlens_k")
     L = load()
-    address, size = _workspace(workspace, 0 if workspace is not None else L.vb200_prefill_packed_workspace_bytes(C.byref(_packed_args(q, k, batch))), q, stream)
+    workspace, address, size = _workspace(workspace, 0 if workspace is not None else L.vb200_prefill_packed_workspace_bytes(C.byref(_packed_args(q, k, batch))), q, stream)
     rc = L.vb200_prefill_packed_fwd(_PACKED.pack(
         _PACKED.size, device, _stream(device, stream), _code(q), batch, Hq, Hkv, D, tq, tk, int(causal), scale, *_view3("q", q, q, (tq, Hq, D)), *_view3("o", o, q, (tq, Hq, D)),
         *_view3("k", k, q, (tk, Hkv, D)), *_view3("v", v, q, (tk, Hkv, D)), _whole("lse", lse, torch.float32, device, tq * Hq),
@@ -291,7 +293,7 @@ def decode_kv4(q, o, cache, *, scale, k_new=None, v_new=None, lse=None, seq_lens
     if device != cache.device:
         raise ValueError(f"decode_kv4: q on {q.device}, cache on {cache.k_codes.device}")
     L = load()
-    address, size = _workspace(workspace, 0 if workspace is not None else L.vb200_decode_kv4_workspace_bytes(C.byref(_decode_args(q, cache, max_len, num_splits))), q, stream)
+    workspace, address, size = _workspace(workspace, 0 if workspace is not None else L.vb200_decode_kv4_workspace_bytes(C.byref(_decode_args(q, cache, max_len, num_splits))), q, stream)
     rc = L.vb200_decode_kv4_fwd(_DECODE.pack(
         _DECODE.size, device, _stream(device, stream), _code(q), B, Hq, cache.Hkv, cache.D, scale, *_view("q", q, q, shape),
         *(_NONE4 if k_new is None else _view("k_new", k_new, q, new)), *(_NONE4 if v_new is None else _view("v_new", v_new, q, new)), *_view("o", o, q, shape),
