@@ -7,10 +7,13 @@ import torch
 
 
 class OnDevice(torch.Tensor):
-    """A CPU tensor that calls itself one of device 0."""
+    """A CPU tensor that calls itself one of device 0, and that knows which streams it was recorded on."""
 
     def get_device(self):
         return 0
+
+    def record_stream(self, stream):
+        self.recorded = getattr(self, "recorded", []) + [stream]
 
 
 def zeros(*shape, dtype=torch.bfloat16):
@@ -74,3 +77,44 @@ def test_the_workspace_lives_through_the_call(serving, monkeypatch, call):
     call(serving)
     assert alive == [[True]]
     assert made[0]() is None
+
+
+class Streams:
+    """torch.cuda's streams, in so far as allocations ask for them: each notes the stream that is current."""
+
+    def __init__(self, monkeypatch):
+        class Stream:
+            device, cuda_stream = torch.device("cpu"), 0
+
+        class Within:
+            def __init__(self, stream):
+                self.stream = stream
+
+            def __enter__(within):
+                within.before, self.now = self.now, within.stream
+
+            def __exit__(within, *error):
+                self.now = within.before
+        self.main, self.side = Stream(), Stream()
+        self.now, self.made = self.main, []
+        monkeypatch.setattr(torch.cuda, "Stream", Stream)
+        monkeypatch.setattr(torch.cuda, "stream", Within)
+        monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: self.now)
+        for name in ("empty", "empty_like"):
+            def allocate(*args, _whole=getattr(torch, name), **kw):
+                t = _whole(*args, **kw)
+                self.made.append((t, self.now))
+                return t
+            monkeypatch.setattr(torch, name, allocate)
+
+
+def test_an_output_on_another_stream_is_that_streams_memory(serving, monkeypatch):
+    """Pending work of the current stream may still use what it has let go of: an output that another stream writes at once comes from that stream's memory, and
+    what the current stream does with it later is waited for before it is given out again."""
+    streams = Streams(monkeypatch)
+    o = packed_call(serving, stream=streams.side)
+    assert streams.made and all(s is streams.side for _, s in streams.made) and any(t is o for t, _ in streams.made)
+    assert o.recorded == [streams.main] and streams.now is streams.main
+    streams.made.clear()
+    o = packed_call(serving)
+    assert all(s is streams.main for _, s in streams.made) and not hasattr(o, "recorded")

@@ -70,3 +70,28 @@ def test_threads_on_one_stream_without_workspaces(S):
     for want, want_d, got in outs:
         for o, od in got:
             assert torch.equal(o, want) and torch.equal(od, want_d)
+
+
+def test_an_output_on_another_stream_while_the_current_one_is_busy(S):
+    """Memory that the current stream has let go of, and still writes to, is not the output of a call on another stream."""
+    g = torch.Generator(device=DEV).manual_seed(3)
+    lens = [700, 324]
+    q, q2, k, v = randn(g, 1024, 16, 128), randn(g, 1024, 16, 128), randn(g, 1024, 4, 128), randn(g, 1024, 4, 128)
+    cu = int32(np.cumsum([0] + lens))
+    want, want2 = (S.prefill_packed(x, k, v, scale=0.09, cu_seqlens_q=cu) for x in (q, q2))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        old = torch.empty_like(q)
+        torch.cuda._sleep(20_000_000)                        # some 10 ms: the fill below comes after the attention
+        old.fill_(7.0)
+        del old
+        o = S.prefill_packed(q, k, v, scale=0.09, cu_seqlens_q=cu, stream=side)
+        torch.cuda.synchronize()
+        assert torch.equal(o, want)
+        torch.cuda._sleep(20_000_000)
+        used = o + 0                                         # the current stream reads it, and lets go of it before that is done
+        del o
+        again = S.prefill_packed(q2, k, v, scale=0.09, cu_seqlens_q=cu, stream=side)
+        torch.cuda.synchronize()
+        assert torch.equal(used, want) and torch.equal(again, want2)

@@ -224,6 +224,18 @@ def _workspace(nbytes, device, stream, least=None, args=None):
     return torch.empty(least(args), dtype=torch.uint8, device=device)
 
 
+def _output_like(t, stream):
+    """A contiguous output like t for a call on `stream` (None: the current one).  Its memory belongs to that stream: what the current one has let go of may still
+    be in use there.  The current stream, which goes on to use it, is waited for before the memory is given out again."""
+    import torch
+    if stream is None or not isinstance(stream, torch.cuda.Stream):
+        return torch.empty_like(t, memory_format=torch.contiguous_format)
+    with torch.cuda.stream(stream):
+        out = torch.empty_like(t, memory_format=torch.contiguous_format)
+    out.record_stream(torch.cuda.current_stream(t.device))
+    return out
+
+
 def _ptr(t):
     return None if t is None else C.c_void_p(t.data_ptr())
 

@@ -207,9 +207,7 @@ def prefill_packed(q, k, v, o=None, lse=None, *, scale, cu_seqlens_q, cu_seqlens
     """vb200_prefill_packed_fwd: q [total_q, Hq, D], k, v [total_k, Hkv, D], cu_seqlens int32 [batch + 1] on the device, lse [Hq, total_q] fp32.  Returns o."""
     import torch
     if o is None:
-        o = torch.empty_like(q, memory_format=torch.contiguous_format)
-        if stream is not None:
-            o.record_stream(stream)                            # let go of early, it is not the current stream's again before this call is done
+        o = capi._output_like(q, stream)
     (tq, Hq, D), (tk, Hkv, _) = q.shape, k.shape
     device, batch = q.get_device(), cu_seqlens_q.numel() - 1
     if cu_seqlens_k is None and tk < tq:
