@@ -118,3 +118,17 @@ def test_an_output_on_another_stream_is_that_streams_memory(serving, monkeypatch
     streams.made.clear()
     o = packed_call(serving)
     assert all(s is streams.main for _, s in streams.made) and not hasattr(o, "recorded")
+
+
+def test_gradients_on_another_stream_are_that_streams_memory(monkeypatch):
+    """The same for the outputs of the fp32 attention's backward pass."""
+    from vesper_b200 import capi
+    library = Library()
+    monkeypatch.setattr(capi, "load", lambda: library)
+    streams = Streams(monkeypatch)
+    x, lse = zeros(1, 2, 5, 64, dtype=torch.float32), zeros(1, 2, 5, dtype=torch.float32)
+    got = capi.attention_bwd(x, x, x, x, x, lse, scale=0.1, stream=streams.side)
+    assert library.seen == ["vb200_attention_bwd"] and len(streams.made) == 4 and all(s is streams.side for _, s in streams.made)
+    assert all(g.recorded == [streams.main] and g.shape == x.shape and g.is_contiguous() for g in got)
+    streams.made.clear()
+    assert not any(hasattr(g, "recorded") for g in capi.attention_bwd(x, x, x, x, x, lse, scale=0.1)) and all(s is streams.main for _, s in streams.made)

@@ -95,3 +95,25 @@ def test_an_output_on_another_stream_while_the_current_one_is_busy(S):
         again = S.prefill_packed(q2, k, v, scale=0.09, cu_seqlens_q=cu, stream=side)
         torch.cuda.synchronize()
         assert torch.equal(used, want) and torch.equal(again, want2)
+
+
+def test_gradients_on_another_stream_while_the_current_one_is_busy(S):
+    """The same for the outputs of the fp32 attention's backward pass."""
+    from vesper_b200 import capi
+    g = torch.Generator(device=DEV).manual_seed(4)
+    q, k, v, do = (randn(g, 1, 8, 700, 64, dtype=torch.float32) for _ in range(4))
+    o, lse = torch.empty_like(q), torch.empty(1, 8, 700, device=DEV)
+    capi.prefill(q, k, v, o, lse, scale=0.125)
+    want = capi.attention_bwd(do, q, k, v, o, lse, scale=0.125)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        old = [torch.empty_like(q) for _ in range(3)]
+        torch.cuda._sleep(20_000_000)
+        for t in old:
+            t.fill_(7.0)
+        del old, t
+        got = capi.attention_bwd(do, q, k, v, o, lse, scale=0.125, stream=side)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        del got

@@ -356,7 +356,6 @@ def profile_read():
 def attention_bwd(d_out, q, k, v, out, lse, *, scale, causal=True, stream=None, workspace=None):
     """fp32 contiguous [B,H,N,D] tensors; returns (dq, dk, dv).  A workspace smaller than vb200_attention_bwd_workspace_bytes, B*H*N floats at least,
     runs on the CUDA cores."""
-    import torch
     B, H, N, D = q.shape
     a = AttnBwdArgs()
     a.struct_size = C.sizeof(AttnBwdArgs)
@@ -364,10 +363,7 @@ def attention_bwd(d_out, q, k, v, out, lse, *, scale, causal=True, stream=None, 
     a.stream = _stream_ptr(stream)
     a.dtype = dtype_code(q)
     a.B, a.H, a.N, a.D, a.causal, a.scale = B, H, N, D, int(causal), scale
-    dq, dk, dv = torch.empty_like(q), torch.empty_like(q), torch.empty_like(q)
-    if stream is not None and isinstance(stream, torch.cuda.Stream):
-        for t in (dq, dk, dv):
-            t.record_stream(stream)                        # let go of early, they are not the current stream's again before this call is done
+    dq, dk, dv = (_output_like(q, stream) for _ in range(3))
     for name, t in (("d_out", d_out), ("q", q), ("k", k), ("v", v), ("out", out), ("lse", lse), ("dq", dq), ("dk", dk), ("dv", dv)):
         assert t.is_contiguous()
         setattr(a, name, _ptr(t))
