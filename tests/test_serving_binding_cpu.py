@@ -16,8 +16,8 @@ class OnDevice(torch.Tensor):
         self.recorded = getattr(self, "recorded", []) + [stream]
 
 
-def zeros(*shape, dtype=torch.bfloat16):
-    return torch.zeros(*shape, dtype=dtype).as_subclass(OnDevice)
+def zeros(*shape, dtype=torch.bfloat16, kind=OnDevice):
+    return torch.zeros(*shape, dtype=dtype).as_subclass(kind)
 
 
 class Library:
@@ -47,19 +47,37 @@ def serving(monkeypatch):
     del serving_capi.library
 
 
-def packed_call(serving, **kw):
-    q, k = zeros(6, 4, 64), zeros(6, 2, 64)
-    return serving.prefill_packed(q, k, k, scale=0.1, cu_seqlens_q=zeros(3, dtype=torch.int32), **kw)
+def packed_call(serving, kind=OnDevice, **kw):
+    q, k = zeros(6, 4, 64, kind=kind), zeros(6, 2, 64, kind=kind)
+    kw = {"cu_seqlens_q": zeros(3, dtype=torch.int32, kind=kind), **kw}
+    return serving.prefill_packed(q, k, k, scale=0.1, **kw)
 
 
-def a_cache(serving):
-    u = lambda n: zeros(2, 2, 16, n, dtype=torch.uint8)  # noqa: E731
+def a_cache(serving, kind=OnDevice):
+    u = lambda n: zeros(2, 2, 16, n, dtype=torch.uint8, kind=kind)  # noqa: E731
     return serving.Kv4Cache(k_codes=u(32), v_codes=u(32), k_scales=u(2), v_scales=u(2))
 
 
-def decode_call(serving, **kw):
-    q = zeros(2, 4, 1, 64)
-    return serving.decode_kv4(q, torch.empty_like(q), a_cache(serving), scale=0.1, uniform_len=3, **kw)
+def decode_call(serving, kind=OnDevice, **kw):
+    q = zeros(2, 4, 1, 64, kind=kind)
+    return serving.decode_kv4(q, torch.empty_like(q), a_cache(serving, kind), scale=0.1, **{"uniform_len": 3, **kw})
+
+
+def norm_call(serving, kind=OnDevice, **kw):
+    return serving.qk_norm_rope(zeros(2, 4, 3, 64, kind=kind), zeros(2, 2, 3, 64, kind=kind), **{"eps": 1e-6, "theta": 1e4, **kw})
+
+
+def append_call(serving, kind=OnDevice, **kw):
+    k = zeros(2, 2, 3, 64, kind=kind)
+    a_cache(serving, kind).append(k, k, **kw)
+
+
+def read_call(serving, kind=OnDevice, **kw):
+    k = zeros(2, 2, 3, 64, kind=kind)
+    a_cache(serving, kind).read(k, k, **kw)
+
+
+CALLS = [norm_call, packed_call, append_call, read_call, decode_call]
 
 
 @pytest.mark.parametrize("call", [packed_call, decode_call])
@@ -132,3 +150,21 @@ def test_gradients_on_another_stream_are_that_streams_memory(monkeypatch):
     assert all(g.recorded == [streams.main] and g.shape == x.shape and g.is_contiguous() for g in got)
     streams.made.clear()
     assert not any(hasattr(g, "recorded") for g in capi.attention_bwd(x, x, x, x, x, lse, scale=0.1)) and all(s is streams.main for _, s in streams.made)
+
+
+@pytest.mark.parametrize("call", CALLS)
+def test_tensors_of_the_cpu_are_refused(serving, monkeypatch, call):
+    """Their addresses would go to a kernel: get_device() is -1 for all of them, which the library takes for the current device."""
+    monkeypatch.setattr(serving.capi, "inv_freq", lambda theta, D: [1.0] * (D // 2))
+    call(serving)
+    assert len(serving.library.seen) == 1
+    with pytest.raises(ValueError, match="CUDA"):
+        call(serving, kind=torch.Tensor)
+    assert len(serving.library.seen) == 1
+
+
+def test_workspaces_of_the_cpu_are_refused(serving):
+    with pytest.raises(ValueError, match="CUDA"):
+        serving.prefill_packed_workspace(torch.zeros(6, 4, 64, dtype=torch.bfloat16), torch.zeros(6, 2, 64, dtype=torch.bfloat16), batch=2)
+    with pytest.raises(ValueError, match="CUDA"):
+        serving.decode_kv4_workspace(torch.zeros(2, 4, 1, 64, dtype=torch.bfloat16), a_cache(serving, torch.Tensor))

@@ -83,6 +83,15 @@ def _code(t):
     return _TYPES[t.dtype]
 
 
+def _device(name, t):
+    """The device that a call runs on: its first tensor's, which the others are compared with.  (-1, as all tensors of the CPU have it, would be the current device
+    to the library.)"""
+    device = t.get_device()
+    if device < 0:
+        raise ValueError(f"{name}: expected a tensor of a CUDA device, got one on {t.device}")
+    return device
+
+
 def _stream(device, stream):
     """The raw handle of `stream`, or of the device's current one."""
     if stream is not None:
@@ -150,7 +159,7 @@ def qk_norm_rope(q, k, v=None, *, eps=None, q_weight=None, k_weight=None, theta=
     if some is None:
         raise ValueError("qk_norm_rope: one of q, k, v must be given")
     B, _, T, D = some.shape
-    device, scatter = some.get_device(), rows is not None
+    device, scatter = _device("qk_norm_rope", some), rows is not None
     kv = k if k is not None else v
     Hq, Hkv = q.shape[1] if q is not None else 0, kv.shape[1] if kv is not None else 0
     q_out = q if q_out is None else q_out
@@ -194,7 +203,7 @@ def qk_norm_rope(q, k, v=None, *, eps=None, q_weight=None, k_weight=None, theta=
 
 
 def _packed_args(q, k, batch):
-    return PackedArgs(struct_size=C.sizeof(PackedArgs), device=q.get_device(), dtype=_code(q), batch=batch, Hq=q.shape[1], Hkv=k.shape[1], D=q.shape[2],
+    return PackedArgs(struct_size=C.sizeof(PackedArgs), device=_device("q", q), dtype=_code(q), batch=batch, Hq=q.shape[1], Hkv=k.shape[1], D=q.shape[2],
                       total_q=q.shape[0], total_k=k.shape[0])
 
 
@@ -206,10 +215,10 @@ def prefill_packed_workspace(q, k, *, batch):
 def prefill_packed(q, k, v, o=None, lse=None, *, scale, cu_seqlens_q, cu_seqlens_k=None, causal=True, workspace=None, stream=None):
     """vb200_prefill_packed_fwd: q [total_q, Hq, D], k, v [total_k, Hkv, D], cu_seqlens int32 [batch + 1] on the device, lse [Hq, total_q] fp32.  Returns o."""
     import torch
+    device, batch = _device("q", q), cu_seqlens_q.numel() - 1
     if o is None:
         o = capi._output_like(q, stream)
     (tq, Hq, D), (tk, Hkv, _) = q.shape, k.shape
-    device, batch = q.get_device(), cu_seqlens_q.numel() - 1
     if cu_seqlens_k is None and tk < tq:
         raise ValueError("prefill_packed: fewer keys than queries need cu_seqlens_k")
     L = load()
@@ -251,7 +260,7 @@ class Kv4Cache:
         if some is None:
             raise ValueError("Kv4Cache: k and v are both missing")
         B, _, T, _ = some.shape
-        shape, device = (B, self.Hkv, T, self.D), some.get_device()
+        shape, device = (B, self.Hkv, T, self.D), _device("k and v", some)
         if device != self.device:
             raise ValueError(f"Kv4Cache: rows on {some.device}, cache on {self.k_codes.device}")
         if seqs is not None and rows is None:
@@ -272,7 +281,7 @@ class Kv4Cache:
 
 
 def _decode_args(q, cache, max_len, num_splits):
-    return DecodeKv4Args(struct_size=C.sizeof(DecodeKv4Args), device=q.get_device(), dtype=_code(q), B=q.shape[0], Hq=q.shape[1], Hkv=cache.Hkv, D=q.shape[3],
+    return DecodeKv4Args(struct_size=C.sizeof(DecodeKv4Args), device=_device("q", q), dtype=_code(q), B=q.shape[0], Hq=q.shape[1], Hkv=cache.Hkv, D=q.shape[3],
                          cache=cache.view, max_len=max_len, num_splits=num_splits)
 
 
@@ -287,7 +296,7 @@ def decode_kv4(q, o, cache, *, scale, k_new=None, v_new=None, lse=None, seq_lens
     """vb200_decode_kv4_fwd: one token per sequence, q and o [B, Hq, 1, D], k_new and v_new [B, Hkv, 1, D] appended first, seq_lens int32 [B] on the device."""
     import torch
     B, Hq = q.shape[0], q.shape[1]
-    device, shape, new = q.get_device(), (B, Hq, 1, cache.D), (B, cache.Hkv, 1, cache.D)
+    device, shape, new = _device("q", q), (B, Hq, 1, cache.D), (B, cache.Hkv, 1, cache.D)
     if device != cache.device:
         raise ValueError(f"decode_kv4: q on {q.device}, cache on {cache.k_codes.device}")
     L = load()
