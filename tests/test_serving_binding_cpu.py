@@ -168,3 +168,26 @@ def test_workspaces_of_the_cpu_are_refused(serving):
         serving.prefill_packed_workspace(torch.zeros(6, 4, 64, dtype=torch.bfloat16), torch.zeros(6, 2, 64, dtype=torch.bfloat16), batch=2)
     with pytest.raises(ValueError, match="CUDA"):
         serving.decode_kv4_workspace(torch.zeros(2, 4, 1, 64, dtype=torch.bfloat16), a_cache(serving, torch.Tensor))
+
+
+def test_arrays_have_to_have_their_shape(serving, monkeypatch):
+    """[T, B] for [B, T] would be read in the wrong order.  One dimension for all is the documented order, and dimensions of one change nothing."""
+    monkeypatch.setattr(serving.capi, "inv_freq", lambda theta, D: [1.0] * (D // 2))
+    i, f = lambda *s: zeros(*s, dtype=torch.int32), lambda *s: zeros(*s, dtype=torch.float32)  # noqa: E731
+    k_cache = zeros(2, 2, 16, 64)
+    to_cache = dict(k_out=k_cache, q_out=zeros(2, 4, 3, 64))
+    right = [(norm_call, dict(positions=i(2, 3))), (norm_call, dict(positions=i(6))), (norm_call, dict(positions=i(2, 3, 1))), (norm_call, dict(q_weight=f(64), k_weight=f(1, 64))),
+             (norm_call, dict(rows=i(2, 3), seqs=i(2, 3), **to_cache)), (packed_call, dict(lse=f(4, 6))), (packed_call, dict(lse=f(24))), (packed_call, dict(cu_seqlens_k=i(3))),
+             (append_call, dict(rows=i(2, 3), seqs=i(2, 3))), (read_call, dict(rows=i(2, 3))), (decode_call, dict(lse=f(2, 4))), (decode_call, dict(lse=f(2, 4, 1))),
+             (decode_call, dict(seq_lens=i(2, 1)))]
+    wrong = [(norm_call, dict(positions=i(3, 2))), (norm_call, dict(positions=i(2, 4))), (norm_call, dict(q_weight=f(8, 8))), (norm_call, dict(rows=i(3, 2), **to_cache)),
+             (norm_call, dict(rows=i(2, 3), seqs=i(3, 2), **to_cache)), (packed_call, dict(lse=f(6, 4))), (packed_call, dict(lse=f(2, 12))), (packed_call, dict(cu_seqlens_k=i(4))),
+             (append_call, dict(rows=i(3, 2))), (append_call, dict(rows=i(2, 3), seqs=i(3, 2))), (read_call, dict(rows=i(3, 2))), (decode_call, dict(lse=f(4, 2))),
+             (decode_call, dict(seq_lens=i(3)))]
+    for call, kw in right:
+        call(serving, **kw)
+    assert len(serving.library.seen) == len(right)
+    for call, kw in wrong:
+        with pytest.raises(ValueError, match="shape"):
+            call(serving, **kw)
+    assert len(serving.library.seen) == len(right)

@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import ctypes as C
+import math
 import struct
 
 from . import capi
@@ -125,18 +126,24 @@ def _view3(name, t, model, shape):
     return t.data_ptr(), 0, s[1], s[0]
 
 
-def _whole(name, t, dtype, device, numel):
+def _same_order(got, shape):
+    """Whether an array of shape `got` lies as one of `shape` does: but for dimensions of one, or in one dimension for all."""
+    long = lambda s: [n for n in s if n != 1]  # noqa: E731
+    return long(got) == long(shape) or (len(got) == 1 and got[0] == math.prod(shape))
+
+
+def _whole(name, t, dtype, device, shape):
     """The address of an array that the kernels read as it lies (0: none)."""
     if t is None:
         return 0
-    if t.dtype is not dtype or t.get_device() != device or t.numel() != numel or not t.is_contiguous():
-        raise ValueError(f"{name}: expected {numel} contiguous {dtype} on device {device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    if t.dtype is not dtype or t.get_device() != device or not t.is_contiguous() or (t.shape != shape and not _same_order(t.shape, shape)):
+        raise ValueError(f"{name}: expected contiguous {dtype} of shape {shape} on device {device}, got {tuple(t.shape)} {t.dtype} on {t.device}, strides {t.stride()}")
     return t.data_ptr()
 
 
-def _rows(rows, seqs, device, tokens, n_seqs, cap):
+def _rows(rows, seqs, device, shape, n_seqs, cap):
     import torch
-    return _whole("rows", rows, torch.int32, device, tokens), _whole("seqs", seqs, torch.int32, device, tokens), n_seqs, cap
+    return _whole("rows", rows, torch.int32, device, shape), _whole("seqs", seqs, torch.int32, device, shape), n_seqs, cap
 
 
 def _workspace(workspace, need, t, stream):
@@ -172,13 +179,13 @@ def qk_norm_rope(q, k, v=None, *, eps=None, q_weight=None, k_weight=None, theta=
         if cache is None:
             raise ValueError("qk_norm_rope: rows need k_out or v_out")
         kv_out_shape = (cache.shape[0], Hkv, cache.shape[2], D)
-        dst = _rows(rows, seqs, device, B * T, cache.shape[0], cache.shape[2])
+        dst = _rows(rows, seqs, device, (B, T), cache.shape[0], cache.shape[2])
     elif seqs is not None:
         raise ValueError("qk_norm_rope: seqs need rows")
     shape_q, shape_kv = (B, Hq, T, D), (B, Hkv, T, D)
     qw = kw = turned = table = 0
     if eps is not None:
-        qw, kw = _whole("q_weight", q_weight, torch.float32, device, D), _whole("k_weight", k_weight, torch.float32, device, D)
+        qw, kw = _whole("q_weight", q_weight, torch.float32, device, (D,)), _whole("k_weight", k_weight, torch.float32, device, (D,))
     if inv_freq is None and theta is not None:
         inv_freq = capi.inv_freq(theta, D)
     if inv_freq is not None:
@@ -195,7 +202,7 @@ def qk_norm_rope(q, k, v=None, *, eps=None, q_weight=None, k_weight=None, theta=
                    *(_NONE4 if q is None else _view("q", q, some, shape_q)), *(_NONE4 if k is None else _view("k", k, some, shape_kv)),
                    *(_NONE4 if v is None else _view("v", v, some, shape_kv)), *(_NONE4 if q_out is None else _view("q_out", q_out, some, shape_q)),
                    *(_NONE4 if k_out is None else _view("k_out", k_out, some, kv_out_shape)), *(_NONE4 if v_out is None else _view("v_out", v_out, some, kv_out_shape)),
-                   int(eps is not None), eps or 0.0, qw, kw, turned, table, start_pos, _whole("positions", positions, torch.int32, device, B * T), *dst)
+                   int(eps is not None), eps or 0.0, qw, kw, turned, table, start_pos, _whole("positions", positions, torch.int32, device, (B, T)), *dst)
     rc = load().vb200_qk_norm_rope(a)
     if rc:
         capi.check(rc)
@@ -225,8 +232,8 @@ def prefill_packed(q, k, v, o=None, lse=None, *, scale, cu_seqlens_q, cu_seqlens
     workspace, address, size = _workspace(workspace, 0 if workspace is not None else L.vb200_prefill_packed_workspace_bytes(C.byref(_packed_args(q, k, batch))), q, stream)
     rc = L.vb200_prefill_packed_fwd(_PACKED.pack(
         _PACKED.size, device, _stream(device, stream), _code(q), batch, Hq, Hkv, D, tq, tk, int(causal), scale, *_view3("q", q, q, (tq, Hq, D)), *_view3("o", o, q, (tq, Hq, D)),
-        *_view3("k", k, q, (tk, Hkv, D)), *_view3("v", v, q, (tk, Hkv, D)), _whole("lse", lse, torch.float32, device, tq * Hq),
-        _whole("cu_seqlens_q", cu_seqlens_q, torch.int32, device, batch + 1), _whole("cu_seqlens_k", cu_seqlens_k, torch.int32, device, batch + 1), address, size))
+        *_view3("k", k, q, (tk, Hkv, D)), *_view3("v", v, q, (tk, Hkv, D)), _whole("lse", lse, torch.float32, device, (Hq, tq)),
+        _whole("cu_seqlens_q", cu_seqlens_q, torch.int32, device, (batch + 1,)), _whole("cu_seqlens_k", cu_seqlens_k, torch.int32, device, (batch + 1,)), address, size))
     if rc:
         capi.check(rc)
     return o
@@ -267,7 +274,7 @@ class Kv4Cache:
             raise ValueError("Kv4Cache: seqs need rows")
         rc = entry(_KV4_ROWS.pack(
             _KV4_ROWS.size, device, _stream(device, stream), _code(some), B, self.Hkv, T, self.D, *(_NONE4 if k is None else _view("k", k, some, shape)),
-            *(_NONE4 if v is None else _view("v", v, some, shape)), *self._fields, start_row, *_rows(rows, seqs, device, B * T, self.seqs, self.cap)))
+            *(_NONE4 if v is None else _view("v", v, some, shape)), *self._fields, start_row, *_rows(rows, seqs, device, (B, T), self.seqs, self.cap)))
         if rc:
             capi.check(rc)
 
@@ -304,7 +311,7 @@ def decode_kv4(q, o, cache, *, scale, k_new=None, v_new=None, lse=None, seq_lens
     rc = L.vb200_decode_kv4_fwd(_DECODE.pack(
         _DECODE.size, device, _stream(device, stream), _code(q), B, Hq, cache.Hkv, cache.D, scale, *_view("q", q, q, shape),
         *(_NONE4 if k_new is None else _view("k_new", k_new, q, new)), *(_NONE4 if v_new is None else _view("v_new", v_new, q, new)), *_view("o", o, q, shape),
-        _whole("lse", lse, torch.float32, device, B * Hq), *cache._fields, _whole("seq_lens", seq_lens, torch.int32, device, B), uniform_len, int(advance_lens), max_len, num_splits,
+        _whole("lse", lse, torch.float32, device, (B, Hq)), *cache._fields, _whole("seq_lens", seq_lens, torch.int32, device, (B,)), uniform_len, int(advance_lens), max_len, num_splits,
         address, size))
     if rc:
         capi.check(rc)
