@@ -191,3 +191,15 @@ def test_arrays_have_to_have_their_shape(serving, monkeypatch):
         with pytest.raises(ValueError, match="shape"):
             call(serving, **kw)
     assert len(serving.library.seen) == len(right)
+
+
+@pytest.mark.parametrize("which", ["q_weight", "k_weight"])
+def test_weights_without_a_norm_are_refused(serving, monkeypatch, which):
+    """They would be left out without a word."""
+    monkeypatch.setattr(serving.capi, "inv_freq", lambda theta, D: [1.0] * (D // 2))
+    with pytest.raises(ValueError, match="eps"):
+        norm_call(serving, eps=None, **{which: zeros(64, dtype=torch.float32)})
+    assert not serving.library.seen
+    norm_call(serving, eps=None)
+    norm_call(serving, eps=0.0, **{which: zeros(64, dtype=torch.float32)})
+    assert len(serving.library.seen) == 2

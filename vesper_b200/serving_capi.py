@@ -184,6 +184,8 @@ def qk_norm_rope(q, k, v=None, *, eps=None, q_weight=None, k_weight=None, theta=
         raise ValueError("qk_norm_rope: seqs need rows")
     shape_q, shape_kv = (B, Hq, T, D), (B, Hkv, T, D)
     qw = kw = turned = table = 0
+    if eps is None and (q_weight is not None or k_weight is not None):
+        raise ValueError("qk_norm_rope: weights need eps, without which there is no norm")
     if eps is not None:
         qw, kw = _whole("q_weight", q_weight, torch.float32, device, (D,)), _whole("k_weight", k_weight, torch.float32, device, (D,))
     if inv_freq is None and theta is not None:
