@@ -19,7 +19,8 @@ extern "C" {
 
 /* Where the tokens of a call go, or come from, in a cache of `seqs` sequences of `cap` rows each: token (b, t) belongs to row rows[b * T + t] of
  * sequence seq_ids[b * T + t] (seq_ids null: sequence b).  A negative row names no place: the token is left out (padding).  A row of cap or above, or a
- * sequence out of [0, seqs), is left out too and sets the status word (VB200_ERR_CACHE_OVERFLOW).  A call may name a place once only. */
+ * sequence out of [0, seqs), is left out too and sets the status word (VB200_ERR_CACHE_OVERFLOW; its detail names the
+ * sequence).  A call may name a place once only. */
 typedef struct vb200_rows {
     const int32_t* rows;         /* device [B, T] contiguous */
     const int32_t* seq_ids;      /* device [B, T] contiguous, or null */

@@ -8,6 +8,7 @@
 #include <string>
 
 #include "kernels.h"
+#include "serving.h"
 
 namespace vb200 {
 
@@ -294,7 +295,8 @@ int vb200_kernel_status_of(int32_t host) {
     if (host == 0) return VB200_OK;
     char buf[96];
     if ((host >> 24) == 2) {
-        std::snprintf(buf, sizeof(buf), "decode: sequence %d is full (token not appended, length not advanced)", host & 0xFFFFFF);
+        if (host & kNoPlace) std::snprintf(buf, sizeof(buf), "rows: sequence %d is not in the cache, or the row named in it (token left out)", static_cast<int>(static_cast<unsigned>(host) << 9) >> 9);
+        else std::snprintf(buf, sizeof(buf), "decode: sequence %d is full (token not appended, length not advanced)", host & 0xFFFFFF);
         return set_detail(VB200_ERR_CACHE_OVERFLOW, buf);
     }
     std::snprintf(buf, sizeof(buf), "kernel wait expired: code %d, site 0x%x", host >> 24, host & 0xFFFFFF);

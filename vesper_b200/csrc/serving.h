@@ -17,6 +17,8 @@ struct RowMap {
 struct Place {
     int seq, row;                          // row < 0: left out
 };
+// Beside code 2 of the status word (a sequence that is full): a place that the cache does not have; the sequence in 23 bits with its sign (beyond them, the ends).
+constexpr int kNoPlace = 0x800000;
 #ifdef __CUDACC__
 // token (b, t) of T per sequence; out-of-range places set the status word and are left out
 __device__ __forceinline__ Place find_place(const RowMap& m, int b, int t, int T, int* status) {
@@ -25,7 +27,7 @@ __device__ __forceinline__ Place find_place(const RowMap& m, int b, int t, int T
     p.row = m.rows[i];
     p.seq = m.seq_ids ? m.seq_ids[i] : b;
     if (p.row >= 0 && (p.row >= m.cap || p.seq < 0 || p.seq >= m.seqs)) {
-        atomicCAS(status, 0, (2 << 24) | (p.seq & 0xFFFFFF));
+        atomicCAS(status, 0, (2 << 24) | kNoPlace | (max(-0x400000, min(p.seq, 0x3FFFFF)) & 0x7FFFFF));
         p.row = -1;
     }
     return p;
