@@ -278,7 +278,8 @@ int vb200_decode_kv4_fwd(const vb200_decode_kv4_args* a) {
         (append && (!view_aligned(used(a->k_new, a->B, a->Hkv, 1), 2) || !view_aligned(used(a->v_new, a->B, a->Hkv, 1), 2))))
         return set_detail(VB200_ERR_ALIGNMENT, "q / k_new / v_new / o base and strides must be 16-byte aligned");
     const Kv4Plan pl = plan_kv4(a);
-    if (pl.units * pl.tiles > INT32_MAX || a->cache.cap >= 1 << 30) return set_detail(VB200_ERR_INVALID_ARG, "4-bit decode: too many rows in one call");
+    // (the tiles of a step, and what rounding them up to equal shares adds, are counted in 32 bits)
+    if (pl.units * pl.tiles + (a->num_splits > 0 ? 0 : pl.ctas) > INT32_MAX || a->cache.cap >= 1 << 30) return set_detail(VB200_ERR_INVALID_ARG, "4-bit decode: too many rows in one call");
     if (!a->workspace || a->workspace_bytes < pl.total) return set_detail(VB200_ERR_WORKSPACE, "decode workspace too small (see vb200_decode_kv4_workspace_bytes)");
     if (reinterpret_cast<uintptr_t>(a->workspace) % 256 != 0) return set_detail(VB200_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
     DeviceGuard g;
