@@ -8,6 +8,7 @@
 // sum the squares with shuffles.  A CTA takes a few tokens and a share of their heads: the angles of a token are computed once
 // per CTA, while its first rows are on their way, and read from shared memory by all of its heads; the rows of a packed projection lie next to each other.
 // 8191 tokens of 32 + 8 heads of 128, bf16: 34 us, 4.9 TB/s, issue slots 60 % busy with shuffles and reads of the angles; 65536 tokens 228 us, 5.9 TB/s.
+// fp32: 8191 tokens 64.5 us, 5.2 TB/s; 32768 tokens 226 us, 5.9 TB/s.
 #include "hybrid.cuh"
 #include "serving.h"
 
@@ -44,9 +45,9 @@ template <> struct Row8<float> {
     __device__ void set(const float (&f)[8]) { a = make_float4(f[0], f[1], f[2], f[3]); b = make_float4(f[4], f[5], f[6], f[7]); }
 };
 
-// (cos, sin) of position * inv_freq, given inv_freq as a fraction of a turn in 64 bits: the product's whole turns fall off the top, so that what is left is
-// good to 2^-33 of a turn at any position.  (In double precision, brought into [-pi, pi], the angles took as long as everything else: 8191 tokens of
-// 32 + 8 heads of 128 41 us, with 4 tokens per CTA 57.)
+// (cos, sin) of position * inv_freq, given inv_freq as a fraction of a turn in 64 bits: the product's whole turns fall off the top, and what is left is good to
+// 2^-33 of a turn at any position; its upper half as a float is rounded by up to 2^-26 of a turn more (at half a turn, less nearer to zero).  (In double
+// precision, brought into [-pi, pi], the angles took as long as everything else: 8191 tokens of 32 + 8 heads of 128 41 us, with 4 tokens per CTA 57.)
 __device__ __forceinline__ float2 turn_of(int position, unsigned long long fraction) {
     const long long t = static_cast<long long>(static_cast<unsigned long long>(static_cast<long long>(position)) * fraction);
     float sn, cs;
@@ -222,11 +223,12 @@ template <typename T, int LANES>
 int launch_t(cudaStream_t s, const QkNormRopeParams& p) {
     const int heads = (p.q.ptr ? p.Hq : 0) + (p.k.ptr ? p.Hkv : 0) + (p.v.ptr ? p.Hkv : 0);
     const long long total = static_cast<long long>(p.B) * p.T;
-    // One round of the CTAs that fit (four per SM) as long as a CTA's share is at most 16 tokens, and then rounds of that.
+    // Four CTAs per SM as long as a CTA's share is at most 16 tokens, and then more: one round of those that fit for 16-bit types.  fp32 rows leave room for two per
+    // SM, and take two rounds: 8191 tokens of 32 + 8 heads of 128 64.5 us (68.6 in one round of two per SM; 1200 tokens 21.5 and 19.5).
     const long long fit = 4LL * device_sm_count();
     const int tokens = static_cast<int>(std::min<long long>(kMaxTokens, (total + fit - 1) / fit));
     const long long blocks = (total + tokens - 1) / tokens;
-    long long shares = (296 + blocks - 1) / blocks;
+    long long shares = (2LL * device_sm_count() + blocks - 1) / blocks;     // of the heads, where the tokens make fewer CTAs than two per SM
     if (shares > heads) shares = heads;
     const int per = static_cast<int>((heads + shares - 1) / shares);
     const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>((heads + per - 1) / per));
