@@ -1,4 +1,4 @@
-"""Packed attention on values that are not finite, where the columns of a tile of scores do not all take the same path; 4-bit decode on queries of nothing."""
+"""Packed attention on values that are not finite, in every column of a block of scores; 4-bit decode on queries of nothing."""
 import math
 
 import numpy as np

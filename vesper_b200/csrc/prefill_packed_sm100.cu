@@ -20,7 +20,10 @@
 // The last block of a tile takes only the columns and rows of V, by 16, that a row of it can see.  The rows of V behind the sequence in its last
 // 16 are another sequence's, or nobody's: they are cleared in shared memory, since a weight of zero does not silence a NaN.
 // What bounds it: the softmax and the products of a tile in turn (long portions: tensor pipe 67 %, special function unit 59 %).  Causal, 32 heads on 8 of 128: 24
-// prompts of 16-4057 tokens 473 us, 1092 TFLOP/s; not causal: 8192 tokens 828 us, 1327 TFLOP/s, with 32 key heads of 64 738 us, 745 TFLOP/s.
+// prompts of 16-4057 tokens 477 us, 1085 TFLOP/s (557 us where calls before it keep the card at its power limit); not causal: 8192 tokens 828 us, 1327 TFLOP/s, with
+// 32 key heads of 64 742 us, 741 TFLOP/s (one after the other, at the power limit, 800-925 us).
+// All weights come from the special function unit.  (One pair in eight from a polynomial on the FMA pipe gains nothing as long as it keeps NaN: 812 us for the
+// 8192 tokens at a clock where this takes 802.)
 // Every wait is bounded (mbar_wait); on expiry the CTA drains and returns with the status word set.
 #include "hybrid.cuh"
 #include "serving.h"
@@ -218,7 +221,6 @@ template <int D>
 struct Cfg {
     static constexpr int kN = D == 128 ? 80 : 112;               // keys of a block
     static constexpr int kStages = D == 128 ? 6 : 8;             // key / value slots
-    static constexpr int kOnFma = 1;                             // of 8 pairs of weights: 1327 TFLOP/s at 8192 x 8192 keys, 0 gives 1280 and 2 1267
     static constexpr int kHalves = D / 64;                       // 64-column (128-byte) boxes per row
     static constexpr int kQHalf = kBlockM * 128, kQTile = kHalves * kQHalf;
     static constexpr int kKvHalf = kN * 128, kKvTile = kHalves * kKvHalf;
@@ -243,27 +245,6 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
         "selp.b32 %0, 1, 0, p;\n\t}"
         : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
     return ok != 0;
-}
-
-// 2^x on the FMA pipe for two numbers: x = n + f with n the nearest whole number (Cody-Waite), a polynomial of degree 4 for 2^f on [-1/2, 1/2] (fitted for
-// the least relative error, 2.6e-6), times 2^n.  n is -127 at least, for which the bits of 2^n are those of zero: x below -126.5, -infinity too, gives 0.  A NaN
-// stays one, since 2^n is a factor; n added to the exponent bits would make it the largest finite number.
-__device__ __forceinline__ float2 exp2_fma(float2 x) {
-    float a, b;
-    asm("max.NaN.f32 %0, %1, 0fC2FE0000;" : "=f"(a) : "f"(x.x));             // -127; a NaN stays one
-    asm("max.NaN.f32 %0, %1, 0fC2FE0000;" : "=f"(b) : "f"(x.y));
-    x = make_float2(a, b);
-    constexpr float kMagic = 12582912.0f;                                    // 1.5 * 2^23: the sum's last bits are n
-    const float2 z = __fadd2_rn(x, make_float2(kMagic, kMagic));
-    const float2 n = __fadd2_rn(z, make_float2(-kMagic, -kMagic));
-    const float2 f = __ffma2_rn(n, make_float2(-1.0f, -1.0f), x);
-    float2 y = make_float2(0.0095701f, 0.0095701f);
-    y = __ffma2_rn(y, f, make_float2(0.05591786f, 0.05591786f));
-    y = __ffma2_rn(y, f, make_float2(0.24024745f, 0.24024745f));
-    y = __ffma2_rn(y, f, make_float2(0.69312181f, 0.69312181f));
-    y = __ffma2_rn(y, f, make_float2(0.99999926f, 0.99999926f));
-    // (two products instead of one of two numbers: head_dim 64, 8192 x 8192 keys, 738 us instead of 774)
-    return make_float2(y.x * __uint_as_float((__float_as_uint(z.x) << 23) + 0x3F800000u), y.y * __uint_as_float((__float_as_uint(z.y) << 23) + 0x3F800000u));
 }
 
 // The item of this CTA where no list is made: found by one warp, 32 sequences at a time.  Returns whether there is one.
@@ -639,12 +620,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __gri
                 const float2 sc2 = make_float2(scale_log2, scale_log2), nm2 = make_float2(-zero, -zero);
                 wait_taken();
                 if (!ok) break;
-                auto weigh = [&](int c, auto on_fma) {                      // columns [16 c, 16 c + 16); of each 8 pairs, the last `on_fma` off the special function unit
+                auto weigh = [&](int c) {                                   // columns [16 c, 16 c + 16)
                     uint32_t pk[8];
 #pragma unroll
                     for (int i = 0; i < 16; i += 2) {
                         const float2 e = __ffma2_rn(make_float2(__uint_as_float(s[16 * c + i]), __uint_as_float(s[16 * c + i + 1])), sc2, nm2);
-                        const float2 pp = i / 2 >= 8 - decltype(on_fma)::value ? exp2_fma(e) : make_float2(fast_exp2(e.x), fast_exp2(e.y));
+                        const float2 pp = make_float2(fast_exp2(e.x), fast_exp2(e.y));
                         rs[(i >> 1) & 3] = __fadd2_rn(rs[(i >> 1) & 3], pp);
                         pk[i >> 1] = Elem<T>::pack2(pp.x, pp.y);
                     }
@@ -652,12 +633,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_packed_kernel(const __gri
                 };
                 if (!masked) {
 #pragma unroll
-                    for (int c = 0; c < C::kN / 16; ++c) weigh(c, std::integral_constant<int, C::kOnFma>());
+                    for (int c = 0; c < C::kN / 16; ++c) weigh(c);
                 } else {
 #pragma unroll
                     for (int c = 0; c < C::kN / 16; ++c) {
                         if (c * 16 >= rest) break;
-                        weigh(c, std::integral_constant<int, 0>());
+                        weigh(c);
                     }
                 }
                 tmem_st_wait();
