@@ -1,7 +1,8 @@
 /*
  * vesper_b200 -- C ABI, operators of a serving batch: norms of queries and keys with the position rotation in one pass, attention over packed
  * prompts of different lengths, and a key / value cache held in 4 bits with the attention that reads it.  The conventions of vesper_b200.h hold:
- * borrowed pointers, nothing allocated, the caller's stream, no synchronisation, status codes.  The reference has none of these operators; they stand
+ * borrowed pointers, nothing allocated, the caller's stream, no synchronisation, status codes; a workspace serves one call at a time, so that calls that may run
+ * at once (on two streams, in two graphs) need one each.  The reference has none of these operators; they stand
  * beside the ones that replace its apply_rotary_emb (src/nn/functional.cpp:424-494), KVCache::update (src/nn/transformer.cpp:56-93) and
  * scaled_dot_product_attention (src/nn/functional.cpp:370-422).
  *

@@ -19,7 +19,7 @@
 // prompts of 16-4057 tokens, tensor pipe busy 49 %, the softmax and the products of a tile waiting for each other.)
 // The last block of a tile takes only the columns and rows of V, by 16, that a row of it can see.  The rows of V behind the sequence in its last
 // 16 are another sequence's, or nobody's: they are cleared in shared memory, since a weight of zero does not silence a NaN.
-// What bounds it: the softmax and the products of a tile in turn (long portions: tensor pipe 67 %, special function unit 59 %).  Causal, 32 heads on 8 of 128: 24
+// What bounds it: the softmax and the products of a tile in turn (long portions: tensor pipe 67 %, special function unit 67 %).  Causal, 32 heads on 8 of 128: 24
 // prompts of 16-4057 tokens 477 us, 1085 TFLOP/s (557 us where calls before it keep the card at its power limit); not causal: 8192 tokens 828 us, 1327 TFLOP/s, with
 // 32 key heads of 64 742 us, 741 TFLOP/s (one after the other, at the power limit, 800-925 us).
 // All weights come from the special function unit.  (One pair in eight from a polynomial on the FMA pipe gains nothing as long as it keeps NaN: 812 us for the

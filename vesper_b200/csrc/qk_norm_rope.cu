@@ -8,7 +8,7 @@
 // sum the squares with shuffles.  A CTA takes a few tokens and a share of their heads: the angles of a token are computed once
 // per CTA, while its first rows are on their way, and read from shared memory by all of its heads; the rows of a packed projection lie next to each other.
 // 8191 tokens of 32 + 8 heads of 128, bf16: 34 us, 4.9 TB/s, issue slots 60 % busy with shuffles and reads of the angles; 65536 tokens 228 us, 5.9 TB/s.
-// fp32: 8191 tokens 64.5 us, 5.2 TB/s; 32768 tokens 226 us, 5.9 TB/s.
+// fp32, a call alone on a cold L2 (bf16 so: 40 us): 8191 tokens 64.5 us, 5.2 TB/s; 32768 tokens 226 us, 5.9 TB/s.
 #include "hybrid.cuh"
 #include "serving.h"
 
