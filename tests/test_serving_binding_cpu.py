@@ -203,3 +203,24 @@ def test_weights_without_a_norm_are_refused(serving, monkeypatch, which):
     norm_call(serving, eps=None)
     norm_call(serving, eps=0.0, **{which: zeros(64, dtype=torch.float32)})
     assert len(serving.library.seen) == 2
+
+
+def test_what_is_allocated_for_a_stream_of_another_library_is_that_streams(serving, monkeypatch):
+    """Any object with a `cuda_stream` names a stream; the memory of a call on it is not the current stream's."""
+    streams = Streams(monkeypatch)
+    theirs, default = type("Theirs", (), {"cuda_stream": 0x50})(), type("Theirs", (), {"cuda_stream": 0})()
+
+    class External(type(streams.side)):
+        def __init__(self, handle, device=None):
+            assert handle                                    # (torch makes a new stream of a handle of zero)
+            self.cuda_stream = handle
+    monkeypatch.setattr(torch.cuda, "ExternalStream", External)
+    monkeypatch.setattr(torch.cuda, "default_stream", lambda device=None: streams.main)
+    for call in (packed_call, decode_call):
+        streams.made.clear()
+        call(serving, stream=theirs)
+        mine = [s for t, s in streams.made if t.dtype is torch.uint8 or call is packed_call]
+        assert mine and all(s.cuda_stream == 0x50 for s in mine)
+        streams.made.clear()
+        call(serving, stream=default)
+        assert all(s is streams.main for _, s in streams.made)

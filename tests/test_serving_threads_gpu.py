@@ -117,3 +117,24 @@ def test_gradients_on_another_stream_while_the_current_one_is_busy(S):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
         del got
+
+
+def test_a_stream_of_another_library(S):
+    """An object with a `cuda_stream` alone: what the call allocates is that stream's, while the current one writes over what it has let go of."""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    lens = [700, 324]
+    q, k, v = randn(g, 1024, 16, 128), randn(g, 1024, 4, 128), randn(g, 1024, 4, 128)
+    cu = int32(np.cumsum([0] + lens))
+    want = S.prefill_packed(q, k, v, scale=0.09, cu_seqlens_q=cu)
+    side = torch.cuda.Stream()
+    theirs = type("Theirs", (), {"cuda_stream": side.cuda_stream})()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)
+        got = S.prefill_packed(q, k, v, scale=0.09, cu_seqlens_q=cu, stream=theirs)
+        for nbytes in (1 << 10, 1 << 14, 1 << 18, 1 << 20, 4 << 20):
+            torch.empty(nbytes, dtype=torch.uint8, device=DEV).fill_(255)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+        del got

@@ -209,12 +209,20 @@ def _stream_ptr(stream):
     return C.c_void_p(s.cuda_stream)
 
 
+def _torch_stream(stream, device):
+    """The stream that any object with a `cuda_stream` names, as torch's own."""
+    import torch
+    if isinstance(stream, torch.cuda.Stream):
+        return stream
+    return torch.cuda.ExternalStream(stream.cuda_stream, device=device) if stream.cuda_stream else torch.cuda.default_stream(device)
+
+
 def _workspace(nbytes, device, stream, least=None, args=None):
     """Bytes that belong to `stream` (None: the current one): torch gives their memory to later work of that stream only.  least(args) bytes where the
     device has no room for all."""
     import torch
-    if stream is not None and isinstance(stream, torch.cuda.Stream):
-        with torch.cuda.stream(stream):
+    if stream is not None:
+        with torch.cuda.stream(_torch_stream(stream, device)):
             return _workspace(nbytes, device, None, least, args)
     try:
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
@@ -228,9 +236,9 @@ def _output_like(t, stream):
     """A contiguous output like t for a call on `stream` (None: the current one).  Its memory belongs to that stream: what the current one has let go of may still
     be in use there.  The current stream, which goes on to use it, is waited for before the memory is given out again."""
     import torch
-    if stream is None or not isinstance(stream, torch.cuda.Stream):
+    if stream is None:
         return torch.empty_like(t, memory_format=torch.contiguous_format)
-    with torch.cuda.stream(stream):
+    with torch.cuda.stream(_torch_stream(stream, t.device)):
         out = torch.empty_like(t, memory_format=torch.contiguous_format)
     out.record_stream(torch.cuda.current_stream(t.device))
     return out
